@@ -95,6 +95,12 @@ _SIGS = {
     "hgsr_anchor_prefilter": (I, [I, P, P, P, I, P, P, I, I, F, F, F, P, P, P, F, F, F, I, P, P]),
     "hgsr_activate_fwd": (I, [I64, P, P, P, P, P]),
     "hgsr_activate_bwd": (I, [I64, P, P, P, P, P, P, P]),
+    "hgsr_embed_fwd": (I, [I64, I64, I64, P, I, I64, P, I, I64, F, P, I, P]),
+    "hgsr_embed_bwd_ws_bytes": (SZ, [I64, I64, I64]),
+    "hgsr_embed_bwd": (I, [I64, I64, I64, P, I, I64, P, I, I64, F, P, I, I64, I, P, SZ, P]),
+    "hgsr_rowcache_write_ws_bytes": (SZ, [I64, I64, I]),
+    "hgsr_rowcache_write": (I, [I64, I64, I64, I, I, P, I, I64, P, I, I64, P, I64, P, I64, P, SZ, P]),
+    "hgsr_rowcache_read": (I, [I64, I64, I64, I, I, P, I64, P, I64, P, I, I64, P, I, P]),
     "hgsr_timing_enable": (I, [I]),
     "hgsr_timing_reset": (I, []),
     "hgsr_timing_only": (I, [ct.c_char_p]),
@@ -131,6 +137,14 @@ def call(name, *args):
     if st != 0:
         msg = lib().hgsr_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed ({st}): {msg}")
+
+
+def call_on(dev, name, *args):
+    """call() with `dev` as the current device and its current torch stream as the last argument."""
+    if dev.index == torch.cuda.current_device():
+        return call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    with torch.cuda.device(dev):
+        return call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
 
 
 def kernel_time(kernel: str):

@@ -14,8 +14,9 @@ anchors to the fused HIP kernels instead of the ~10 torch launches of
   object itself and returns the same 8-tuple, so a maintainer can bind it in place of
   `BasicModel.generate_neural_gaussians` (INTEGRATION.md).
 
-Supported: feat_dim 32, view_dim 0 or 3, appearance_dim 0, dist2level != 'progressive'
-(smooth_complement = 1), RGB or SH colours; anything else raises NotImplementedError.
+Supported: feat_dim 32, view_dim 0 or 3, any appearance_dim, dist2level != 'progressive'
+(smooth_complement = 1), RGB or SH colours; anything else raises NotImplementedError.  The anchor
+features may lie in an 8-bit row cache (rowcache.py) when a model is only rendered.
 There is no CPU path: inputs must be HIP device tensors.
 """
 from __future__ import annotations
@@ -272,15 +273,34 @@ def set_early_grad_hook(fn):
     _EARLY_GRAD[0] = fn
 
 
+def _decode_cached(anchor, feat, offset, scaling_raw, vis_idx):
+    """The visible anchors' arrays, compacted, with the features read back from their row cache."""
+    from .embedding import embedding
+    from .rowcache import rowcache_read
+    if isinstance(vis_idx, VisibleIndex):
+        vi = vis_idx
+        vis_idx = vi.buf[:int(vi.counts[1].item())]  # the compacted arrays need their length on the host
+        _VIS_CACHE[:] = [(vi.visible, vi.visible._version, vis_idx)]
+    take = lambda t: embedding(_f32(t).reshape(t.shape[0], -1), vis_idx).reshape(-1, *t.shape[1:])
+    return take(anchor), rowcache_read(feat, vis_idx), take(offset), take(scaling_raw)
+
+
 def decode(anchor, feat, offset, scaling_raw, cam_center, mlps, visible=None, view_dim=3, n_offsets=10,
-           color_dim=3):
+           color_dim=3, appearance=None):
     """Fused generate_neural_gaussians on the visible anchors.
 
     mlps: (mlp_opacity, mlp_cov, mlp_color) nn.Sequentials, or a dict with
     '{opacity,cov,color}_{w1,b1,w2,b2}' tensors.  visible: bool mask [A] or int index
     tensor (None = all).  Returns (xyz, offsets, color, opacity, scaling, rot, mask)
-    like the reference (colour [M, color_dim//3, 3] for SH)."""
-    _check_dev(anchor, feat, offset, scaling_raw, cam_center)
+    like the reference (colour [M, color_dim//3, 3] for SH).
+
+    feat: [A, 32], or a rowcache.RowCache of A slots (rendering only: no gradients).
+    appearance: the view's row [appearance_dim] (embedding.embedding of its camera), which the
+    colour head takes behind the features and the view direction: its first weight is
+    [32, 32 + view_dim + appearance_dim].  The row is the same for every anchor of a view, so its
+    product with that weight is added to the head's bias once instead of once per anchor."""
+    cached = isinstance(feat, tuple)
+    _check_dev(anchor, *(feat[:2] if cached else (feat,)), offset, scaling_raw, cam_center)
     if isinstance(mlps, dict):
         weights = [mlps[f"{h}_{n}"] for h in _HEADS for n in ("w1", "b1", "w2", "b2")]
     else:
@@ -290,6 +310,29 @@ def decode(anchor, feat, offset, scaling_raw, cam_center, mlps, visible=None, vi
                 raise NotImplementedError("hgsr decode: MLPs must be Linear -> ReLU -> Linear [-> Tanh]")
             weights += [m[0].weight, m[0].bias, m[2].weight, m[2].bias]
     A = anchor.shape[0]
+    if appearance is not None:
+        w1, b1 = weights[8:10]
+        k = w1.shape[1] - appearance.numel()
+        _check_dev(appearance)
+        if k != weights[0].shape[1]:
+            raise ValueError(f"hgsr decode: an appearance row of {appearance.numel()} does not fit the colour head's "
+                             f"{w1.shape[1]} inputs")
+        weights[8:10] = w1[:, :k], b1 + (w1[:, k:] * appearance.reshape(1, -1)).sum(1)
+    elif weights[8].shape[1] != weights[0].shape[1]:
+        raise ValueError("hgsr decode: the colour head takes an appearance row, and none is given")
+    if cached:
+        if feat[0].shape[0] != A:
+            raise ValueError(f"hgsr decode: a row cache of {feat[0].shape[0]} slots for {A} anchors")
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (anchor, offset, scaling_raw, *weights)):
+            raise NotImplementedError("hgsr decode: cached features are for rendering (torch.no_grad())")
+        if visible is None:
+            from .rowcache import rowcache_read
+            feat = rowcache_read(feat)
+        else:
+            idx = visible if isinstance(visible, VisibleIndex) else visible_index(visible) \
+                if visible.dtype == torch.bool else visible.reshape(-1)
+            anchor, feat, offset, scaling_raw = _decode_cached(anchor, feat, offset, scaling_raw, idx)
+            visible, A = None, anchor.shape[0]
     if visible is None:
         vis_idx = torch.arange(A, dtype=torch.int32, device=anchor.device)
     elif isinstance(visible, VisibleIndex):
@@ -306,17 +349,28 @@ def decode(anchor, feat, offset, scaling_raw, cam_center, mlps, visible=None, vi
     return xyz, offs, color, opac, scaling, rot, mask
 
 
-def generate_neural_gaussians(model, viewpoint_camera, visible_mask=None):
+def generate_neural_gaussians(model, viewpoint_camera, visible_mask=None, appearance_id=None):
     """Drop-in for reference BasicModel.generate_neural_gaussians (scene/basic_model.py:297):
-    returns (xyz, offsets, color, opacity, scaling, rot, active_sh_degree, mask)."""
-    if getattr(model, "appearance_dim", 0) > 0:
-        raise NotImplementedError("hgsr decode: appearance embeddings are not supported")
+    returns (xyz, offsets, color, opacity, scaling, rot, active_sh_degree, mask).
+
+    With model.appearance_dim > 0 the colour head takes the row of model.embedding_appearance (an
+    embedding.Embedding, or an nn.Embedding) named by appearance_id, by default the camera's uid; a
+    number outside the table is a row of zeros."""
     if getattr(model, "dist2level", "floor") == "progressive":
         raise NotImplementedError("hgsr decode: dist2level='progressive' is not supported")
+    dev = model.get_anchor.device
+    appearance = None
+    if getattr(model, "appearance_dim", 0) > 0:
+        from .embedding import embedding
+        table = model.embedding_appearance
+        weight, scale = getattr(table, "embedding", table).weight, getattr(table, "scale", 1.0)
+        uid = viewpoint_camera.uid if appearance_id is None else appearance_id
+        appearance = embedding(weight, torch.full((1,), int(uid), dtype=torch.int64, device=dev), scale,
+                               dtype=torch.float32)[0]
     if visible_mask is None:
-        visible_mask = torch.ones(model.get_anchor.shape[0], dtype=torch.bool, device=model.get_anchor.device)
+        visible_mask = torch.ones(model.get_anchor.shape[0], dtype=torch.bool, device=dev)
     xyz, offs, color, opac, scaling, rot, mask = decode(
         model.get_anchor, model.get_anchor_feat, model.get_offset, model._scaling,
         viewpoint_camera.camera_center, (model.get_opacity_mlp, model.get_cov_mlp, model.get_color_mlp),
-        visible_mask, model.view_dim, model.n_offsets, model.color_dim)
+        visible_mask, model.view_dim, model.n_offsets, model.color_dim, appearance=appearance)
     return xyz, offs, color, opac, scaling, rot, model.active_sh_degree, mask

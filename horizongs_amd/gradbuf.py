@@ -48,6 +48,13 @@ def alloc_key(k, like: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(like)
 
 
+def take(k, shape, dtype):
+    """The registered destination (taken) of the tensor whose key is `k`, or None: for a backward
+    that has neither the tensor nor one like it."""
+    d = _DEST.pop(k, None)
+    return d if d is not None and tuple(d.shape) == tuple(shape) and d.dtype == dtype else None
+
+
 def alloc(like: torch.Tensor) -> torch.Tensor:
     """The output buffer for the gradient of `like` itself."""
     return alloc_key(key(like), like)

@@ -598,6 +598,45 @@ int hgsr_activate_fwd(int64_t N, const float* log_scales, const float* logits, f
 int hgsr_activate_bwd(int64_t N, const float* scales, const float* opacities, const float* v_scales,
                       const float* v_opacities, float* v_log_scales, float* v_logits, hgsr_stream_t stream);
 
+/* ---- Tables of learned rows ----------------------------------------------------------------
+ * Element types of the entries below (the other entries are fp32 throughout). */
+enum { HGSR_F32 = 0, HGSR_F16 = 1, HGSR_BF16 = 2 };
+/* Embedding lookup with scaling (the appearance rows of reference scene/embedding.py:50-79):
+ *   out[i, :] = scale * weight[ids[i], :],  i < n,   rounded once from f32 to otype.
+ * weight: V rows of D elements, `wstride` elements apart (columns contiguous); ids: int32, or
+ * int64 if ids64, `ids_stride` elements apart (0: one id for every row); out [n, D] contiguous.
+ * An id outside [0, V) is padding: its row of out is zeros. */
+int hgsr_embed_fwd(int64_t V, int64_t n, int64_t D, const void* weight, int wtype, int64_t wstride, const void* ids,
+                   int ids64, int64_t ids_stride, float scale, void* out, int otype, hgsr_stream_t stream);
+/* Its gradient, dw[v, :] = scale * sum over i with ids[i] = v of g[i, :], summed in f32 in an
+ * order that the ids alone set (no float atomics: the same bits on every run) and rounded once.
+ * accumulate = 0: every row of dw is written, zeros where no id names it; accumulate = 1: the
+ * sums are added to dw's named rows, the others are neither read nor written.  Padding ids take
+ * no part.  Workspace: hgsr_embed_bwd_ws_bytes (any contents). */
+size_t hgsr_embed_bwd_ws_bytes(int64_t V, int64_t n, int64_t D);
+int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, int gtype, int64_t gstride, const void* ids,
+                   int ids64, int64_t ids_stride, float scale, void* dw, int dwtype, int64_t dwstride, int accumulate,
+                   void* ws, size_t ws_bytes, hgsr_stream_t stream);
+/* 8-bit row cache: slot c holds D codes (codes + c cstride bytes) and ceil(D / group) f32 scales
+ * (scales + c sstride), group = 16, 32, 64 or 128 columns.  With top = 127 (HGSR_INT8) or 448
+ * (HGSR_E4M3: 4-bit exponent, 3-bit mantissa, no infinities), a row x is held as
+ *   s = max(max |x| over the group * (1 / top), 2^-100),  code = x / s rounded to nearest, ties to
+ * even -- s in f32, its product with the f32 number 1 / top rounded once, the quotient exact; a group that holds a NaN or an infinity has s = NaN and codes 0, so
+ * it reads back as NaN.  A row whose slot lies outside [0, capacity) is left out; where a slot
+ * is named twice, the last of its rows stays.  slots = NULL: row i goes to slot i (n <= capacity).
+ * Workspace: hgsr_rowcache_write_ws_bytes (any contents; 0 without slots). */
+enum { HGSR_INT8 = 0, HGSR_E4M3 = 1 };
+size_t hgsr_rowcache_write_ws_bytes(int64_t capacity, int64_t n, int has_slots);
+int hgsr_rowcache_write(int64_t capacity, int64_t n, int64_t D, int group, int format, const void* x, int xtype,
+                        int64_t xstride, const void* slots, int slots64, int64_t slots_stride, void* codes,
+                        int64_t cstride, float* scales, int64_t sstride, void* ws, size_t ws_bytes,
+                        hgsr_stream_t stream);
+/* out[i, c] = code * scale of slot slots[i] (slots = NULL: slot i), the f32 product rounded to
+ * otype; a row of zeros for a slot outside [0, capacity).  out [n, D] contiguous. */
+int hgsr_rowcache_read(int64_t capacity, int64_t n, int64_t D, int group, int format, const void* codes,
+                       int64_t cstride, const float* scales, int64_t sstride, const void* slots, int slots64,
+                       int64_t slots_stride, void* out, int otype, hgsr_stream_t stream);
+
 /* ---- measurement ----------------------------------------------------------
  * Optional per-kernel HIP-event timing used by bench.py (roofline numbers):
  * when enabled, the main kernel of every entry point is bracketed by
