@@ -17,33 +17,28 @@ namespace hgsr {
 
 // ------------------------------------------------------------------------------------- lookup
 
-constexpr int kFwdPer = 4;  // pieces per lane, 256 apart
-
-template <typename WT, typename OT, int VEC>
+template <typename WT, typename OT, typename I, int VEC>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(uint32_t chunks, FastDiv per_row, uint32_t V,
-                                                        const WT* __restrict__ w, int64_t wstride, RowIds ids,
-                                                        int64_t row0, float scale, OT* __restrict__ out) {
-    const uint32_t c0 = xcd_remap(blockIdx.x, gridDim.x) * (256 * kFwdPer) + threadIdx.x;
-    uint32_t col[kFwdPer], id[kFwdPer], row[kFwdPer];
+                                                        const WT* __restrict__ w, int64_t wstride, RowIds<I> ids,
+                                                        int64_t row0, float scale, OT* __restrict__ out, int stream) {
+    const uint32_t c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= chunks) return;
+    const uint32_t r = per_row.div(c), col = (c - r * per_row.d) * VEC;
+    const uint32_t id = ids.get(row0 + r, V);
+    Vec<OT, VEC> o;
+    if (id < V) {
+        const Vec<WT, VEC> x = load_vec<WT, VEC>(w + (int64_t)id * wstride + col);
 #pragma unroll
-    for (int k = 0; k < kFwdPer; ++k) {
-        const uint32_t c = c0 + k * 256;
-        row[k] = per_row.div(c < chunks ? c : 0);
-        col[k] = (c - row[k] * per_row.d) * VEC;
-        id[k] = ids.get(row0 + row[k], V);
+        for (int k = 0; k < VEC; ++k) o.v[k] = (OT)((float)x.v[k] * scale);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) o.v[k] = (OT)0.0f;
     }
-    Vec<WT, VEC> x[kFwdPer];
-#pragma unroll
-    for (int k = 0; k < kFwdPer; ++k)
-        if (c0 + k * 256 < chunks && id[k] < V) x[k] = load_vec<WT, VEC>(w + (int64_t)id[k] * wstride + col[k]);
-#pragma unroll
-    for (int k = 0; k < kFwdPer; ++k) {
-        if (c0 + k * 256 >= chunks) break;
-        Vec<OT, VEC> o;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) o.v[j] = (OT)(id[k] < V ? (float)x[k].v[j] * scale : 0.0f);
-        store_vec<OT, VEC>(out + (row0 + row[k]) * ((int64_t)per_row.d * VEC) + col[k], o);
-    }
+    OT* to = out + (row0 + r) * ((int64_t)per_row.d * VEC) + col;
+    if (stream)
+        stream_vec<OT, VEC>(to, o);
+    else
+        store_vec<OT, VEC>(to, o);
 }
 
 // --------------------------------------------------------------------------- zeros of the table
@@ -56,81 +51,187 @@ struct ZeroPart {
     uint16_t* edge[2];  // what lies before the first and behind the last unit (part 0 only)
     int nedge[2];
 };
-constexpr int kZeroUnits = 2048;  // per workgroup: 32 KB
+constexpr int kZeroUnits = 2048;  // per workgroup and turn: 32 KB
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ void store_zeros(const ZeroPart& z, int64_t block) {
-    const int64_t u0 = block * kZeroUnits + threadIdx.x;
+// workgroup `block` of `blocks`; the zeros go past the caches (16k x 2048 bf16 ids into 65,536 rows:
+// 89 us, 100 us with cached stores, which the sums' reads then have to push out)
+template <int THREADS>
+__device__ __forceinline__ void store_zeros(const ZeroPart& z, int64_t block, int64_t blocks) {
+    for (int64_t u0 = block * kZeroUnits + threadIdx.x; u0 < z.units; u0 += blocks * kZeroUnits) {
 #pragma unroll
-    for (int k = 0; k < kZeroUnits / 256; ++k)
-        if (u0 + k * 256 < z.units) z.p[u0 + k * 256] = make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < kZeroUnits / THREADS; ++k)
+            if (u0 + k * THREADS < z.units)
+                __builtin_nontemporal_store(u32x4{0, 0, 0, 0}, reinterpret_cast<u32x4*>(z.p) + u0 + k * THREADS);
+    }
     if (block == 0 && threadIdx.x < 8) {
         if ((int)threadIdx.x < z.nedge[0]) z.edge[0][threadIdx.x] = 0;
         if ((int)threadIdx.x < z.nedge[1]) z.edge[1][threadIdx.x] = 0;
     }
 }
 
-__global__ __launch_bounds__(256) void zero_kernel(ZeroPart z) { store_zeros(z, blockIdx.x); }
+__global__ __launch_bounds__(256) void zero_kernel(ZeroPart z) { store_zeros<256>(z, blockIdx.x, gridDim.x); }
 
 // ------------------------------------------------------------------------------ sort of (id, i)
-// Up to kRankMost entries: the place of each is the number of entries before it, counted by
-// comparing it with all of them -- n^2 comparisons over the whole chip, in one launch.
-constexpr int kRankMost = 16384;
-constexpr int kRankOwn = 4;      // entries per wave
-constexpr int kRankTile = 2048;  // ids staged in LDS at a time
+// Both forms are radix sorts, least significant digit first.  An entry's place among its wave's
+// entries of one digit: `match` of the lanes that hold the digit, one ballot per bit; the first of
+// them adds their number to the wave's count of the digit.
+template <int MOST>
+__device__ __forceinline__ uint64_t match(uint32_t d, bool on, int bits) {
+    uint64_t same = __ballot(on);
+    if (!on) same = ~same;
+#pragma unroll
+    for (int k = 0; k < MOST; ++k)
+        if (k < bits) {
+            const uint64_t m = __ballot((d >> k) & 1);
+            same &= (d >> k) & 1 ? m : ~m;
+        }
+    return same;
+}
+__device__ __forceinline__ uint64_t below(int lane) { return (1ull << lane) - 1; }
 
-__global__ __launch_bounds__(256) void sort_rank_kernel(uint32_t n, RowIds ids, uint32_t V, uint2* __restrict__ out,
-                                                        uint32_t blocks, ZeroPart zeros) {
-    __shared__ uint32_t key[kRankTile];
-    if (blockIdx.x >= blocks) return store_zeros(zeros, blockIdx.x - blocks);
-    const int lane = threadIdx.x & 63;
-    const uint32_t i0 = __builtin_amdgcn_readfirstlane((blockIdx.x * 4 + (threadIdx.x >> 6)) * kRankOwn);
-    uint32_t mine[kRankOwn], before[kRankOwn] = {};
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {  // inclusive
 #pragma unroll
-    for (int q = 0; q < kRankOwn; ++q)
-        mine[q] = __builtin_amdgcn_readfirstlane(i0 + q < n ? ids.get(i0 + q, V) : 0);
-    for (uint32_t j0 = 0; j0 < n; j0 += kRankTile) {
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kRankTile / 256; ++k) {
-            const uint32_t j = j0 + k * 256 + threadIdx.x;
-            key[k * 256 + threadIdx.x] = j < n ? ids.get(j, V) : ~0u;
-        }
-        __syncthreads();
-        if (j0 + kRankTile <= i0 || j0 >= i0 + kRankOwn) {  // all before or all behind this wave's entries
-            const uint32_t tie = j0 < i0 ? 1 : 0;           // an equal id counts if it comes before
-#pragma unroll 8
-            for (int k = 0; k < kRankTile; k += 64) {
-                const uint32_t v = key[k + lane];
-#pragma unroll
-                for (int q = 0; q < kRankOwn; ++q) before[q] += v < mine[q] + tie;
-            }
-        } else {
-            for (int k = 0; k < kRankTile; k += 64) {
-                const uint32_t v = key[k + lane], j = j0 + k + lane;
-#pragma unroll
-                for (int q = 0; q < kRankOwn; ++q) before[q] += v < mine[q] || (v == mine[q] && j < i0 + q);
-            }
-        }
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(v, d);
+        if (lane >= d) v += o;
     }
+    return v;
+}
+
+// Up to kBucketMost entries: one launch.  The ids are cut into up to 256 ranges, a workgroup each: it
+// reads all ids, keeps the positions of its own in LDS (in order) and counts the smaller ones, which
+// is where its part of the list starts; then it sorts what it kept by the ids' remaining bits.
+// (One workgroup for all: 42 us at 16,384 entries, LDS-bound; counting, for each entry, the ones
+// before it: 36 us of the whole chip.)
+constexpr int kBucketMost = 16384;
+constexpr int kBucketRounds = kBucketMost / 1024;
+constexpr int kBucketLog = 8;
+constexpr int kBucketBits = 8;  // per pass
+
+template <typename I>
+__global__ __launch_bounds__(1024) void sort_bucket_kernel(uint32_t n, RowIds<I> ids, uint32_t V, int shift, int passes,
+                                                           int bits, uint2* __restrict__ out, uint32_t buckets,
+                                                           ZeroPart zeros) {
+    __shared__ uint16_t pos[kBucketMost];
+    __shared__ uint32_t cnt[16][1 << kBucketBits];
+    __shared__ uint32_t wsum[2][16];
+    if (blockIdx.x >= buckets) return store_zeros<1024>(zeros, blockIdx.x - buckets, gridDim.x - buckets);
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+    int rounds = (n + 1023) / 1024;
+    uint32_t base = w * rounds * 64 + lane;  // a wave's entries are consecutive
+    uint32_t k[kBucketRounds], place[kBucketRounds];
+    uint16_t p[kBucketRounds];
 #pragma unroll
-    for (int q = 0; q < kRankOwn; ++q) {
+    for (int r = 0; r < kBucketRounds; ++r)
+        if (r < rounds) k[r] = base + r * 64 < n ? ids.get(base + r * 64, V) : ~0u;
+    uint32_t mine = 0, less = 0;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) before[q] += __shfl_xor(before[q], d);
-        if (lane == q && i0 + q < n) out[before[q]] = make_uint2(mine[q], i0 + q);
+    for (int r = 0; r < kBucketRounds; ++r)
+        if (r < rounds) {
+            mine += __popcll(__ballot(k[r] >> shift == blockIdx.x && k[r] != ~0u));
+            less += __popcll(__ballot(k[r] >> shift < blockIdx.x));
+        }
+    if (lane == 0) {
+        wsum[0][w] = mine;
+        wsum[1][w] = less;
+    }
+    __syncthreads();
+    uint32_t m = 0, start = 0, at = 0;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        if (q < w) at += wsum[0][q];
+        m += wsum[0][q];
+        start += wsum[1][q];
+    }
+    if (m == 0) return;
+#pragma unroll
+    for (int r = 0; r < kBucketRounds; ++r)
+        if (r < rounds) {
+            const bool in = k[r] >> shift == blockIdx.x && k[r] != ~0u;
+            const uint64_t b = __ballot(in);
+            if (in) pos[at + __popcll(b & below(lane))] = (uint16_t)(base + r * 64);
+            at += __popcll(b);
+        }
+    __syncthreads();
+    out += start;
+    rounds = (m + 1023) / 1024;
+    base = w * rounds * 64 + lane;
+    if (passes == 0) {  // a range of one id
+        for (int r = 0; r < rounds; ++r)
+            if (base + r * 64 < m) out[base + r * 64] = make_uint2(blockIdx.x, pos[base + r * 64]);
+        return;
+    }
+    const uint32_t bins = 1u << bits;
+    for (int pass = 0; pass < passes; ++pass) {
+        const int sh = pass * bits;
+#pragma unroll
+        for (int r = 0; r < kBucketRounds; ++r)
+            if (r < rounds) {
+                const bool on = base + r * 64 < m;
+                p[r] = on ? pos[base + r * 64] : 0;
+                k[r] = ids.get(p[r], V);
+            }
+        for (uint32_t b = tid; b < 16 * bins; b += 1024) cnt[b >> bits][b & (bins - 1)] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kBucketRounds; ++r)
+            if (r < rounds) {
+                const bool on = base + r * 64 < m;
+                const uint32_t d = (k[r] >> sh) & (bins - 1);
+                const uint64_t same = match<kBucketBits>(d, on, bits);
+                const int first = __ffsll((unsigned long long)same) - 1;
+                uint32_t old = 0;
+                if (on && lane == first) old = atomicAdd(&cnt[w][d], (uint32_t)__popcll(same));
+                place[r] = __shfl(old, first) + __popcll(same & below(lane));
+            }
+        __syncthreads();
+        // where each wave's entries of a digit go: after all smaller digits and the earlier waves'
+        uint32_t c[16], sum = 0;
+        if ((uint32_t)tid < bins) {
+#pragma unroll
+            for (int q = 0; q < 16; ++q) c[q] = cnt[q][tid];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) sum += c[q];
+        }
+        const uint32_t inc = wave_scan(sum, lane);
+        if (lane == 63) wsum[0][w] = inc;
+        __syncthreads();
+        uint32_t to = inc - sum;
+        for (int q = 0; q < w; ++q) to += wsum[0][q];
+        if ((uint32_t)tid < bins) {
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                cnt[q][tid] = to;
+                to += c[q];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kBucketRounds; ++r)
+            if (r < rounds && base + r * 64 < m) {
+                const uint32_t d = cnt[w][(k[r] >> sh) & (bins - 1)] + place[r];
+                if (pass == passes - 1)
+                    out[d] = make_uint2(k[r], p[r]);
+                else
+                    pos[d] = p[r];
+            }
+        __syncthreads();
     }
 }
 
-// More: least-significant-digit radix sort, digits of up to 11 bits.  Per pass: the tiles' digit
-// counts, their prefix over the tiles, a stable scatter.  The first pass also notes whether the
+// More: digits of up to 11 bits, per pass three launches: the tiles' digit counts, their prefix over
+// the tiles, a stable scatter.  The first pass also notes whether the
 // ids ascend already (a compacted index does): the rest of the sort then ends at once, and the
 // sums read the ids themselves.
 constexpr int kSortRounds = 8;
 constexpr int kSortTile = 256 * kSortRounds;  // entries per workgroup: 4 waves x 8 rounds x 64 lanes
 constexpr int kSortBits = 11;
 
+template <typename I>
 struct SortArgs {
     uint32_t n, V;
-    RowIds ids;
+    RowIds<I> ids;
     const uint2* in;   // nullptr: the first pass, entries from the ids
     uint2* out;
     int shift, bits;
@@ -140,34 +241,37 @@ struct SortArgs {
     uint32_t* ascend;  // [1 + tiles]: the verdict, then the tiles' own
 };
 
-template <bool FIRST>
-__device__ __forceinline__ uint2 sort_entry(const SortArgs& a, uint32_t i) {
+template <bool FIRST, typename I>
+__device__ __forceinline__ uint2 sort_entry(const SortArgs<I>& a, uint32_t i) {
     if (FIRST) return make_uint2(a.ids.get(i, a.V), i);
     return a.in[i];
 }
 
-template <bool FIRST>
-__global__ __launch_bounds__(256) void sort_count_kernel(const SortArgs a, ZeroPart zeros) {
+template <bool FIRST, typename I>
+__global__ __launch_bounds__(256) void sort_count_kernel(const SortArgs<I> a, ZeroPart zeros) {
     __shared__ uint32_t h[1 << kSortBits];
-    if (blockIdx.x >= a.tiles) return store_zeros(zeros, blockIdx.x - a.tiles);
+    if (blockIdx.x >= a.tiles) return store_zeros<256>(zeros, blockIdx.x - a.tiles, gridDim.x - a.tiles);
     if (!FIRST && *a.ascend) return;
     const uint32_t bins = 1u << a.bits, base = blockIdx.x * kSortTile;
-    uint32_t v[kSortRounds], next[kSortRounds];
+    const int lane = threadIdx.x & 63;
+    uint32_t v[kSortRounds], after[kSortRounds];  // after: the first id of the next 64
 #pragma unroll
     for (int k = 0; k < kSortRounds; ++k) {
         const uint32_t i = base + k * 256 + threadIdx.x;
-        if (i < a.n) v[k] = sort_entry<FIRST>(a, i).x;
-        if (FIRST) next[k] = i + 1 < a.n ? a.ids.get(i + 1, a.V) : ~0u;
+        v[k] = i < a.n ? sort_entry<FIRST>(a, i).x : ~0u;
+        if (FIRST) after[k] = lane == 63 && i + 1 < a.n ? a.ids.get(i + 1, a.V) : ~0u;
     }
     for (uint32_t b = threadIdx.x; b < bins; b += 256) h[b] = 0;
     __syncthreads();
     int up = 1;
 #pragma unroll
-    for (int k = 0; k < kSortRounds; ++k)
-        if (base + k * 256 + threadIdx.x < a.n) {
-            atomicAdd(&h[(v[k] >> a.shift) & (bins - 1)], 1u);
-            if (FIRST) up &= v[k] <= next[k];
+    for (int k = 0; k < kSortRounds; ++k) {
+        if (base + k * 256 + threadIdx.x < a.n) atomicAdd(&h[(v[k] >> a.shift) & (bins - 1)], 1u);
+        if (FIRST) {
+            const uint32_t next = __shfl_down(v[k], 1);
+            up &= v[k] <= (lane == 63 ? after[k] : next) || v[k] == ~0u;
         }
+    }
     up = __syncthreads_and(up);
     if (FIRST && threadIdx.x == 0) a.ascend[1 + blockIdx.x] = up;
     for (uint32_t b = threadIdx.x; b < bins; b += 256) a.hist[(size_t)blockIdx.x * bins + b] = h[b];
@@ -175,8 +279,8 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const SortArgs a, ZeroP
 
 // 64 digits per workgroup, a share of the tiles per wave: exclusive prefix of each digit's counts
 // over the tiles, and its total.  The last workgroup of the first pass joins the tiles' verdicts.
-template <bool FIRST>
-__global__ __launch_bounds__(1024) void sort_scan_kernel(const SortArgs a) {
+template <bool FIRST, typename I>
+__global__ __launch_bounds__(1024) void sort_scan_kernel(const SortArgs<I> a) {
     __shared__ uint32_t part[16][64];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t bins = 1u << a.bits, bin = blockIdx.x * 64 + lane;
@@ -218,11 +322,11 @@ __global__ __launch_bounds__(1024) void sort_scan_kernel(const SortArgs a) {
     if (w == 0 && bin < bins) a.total[bin] = carry;
 }
 
-template <bool FIRST>
-__global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs a, ZeroPart zeros) {
+template <bool FIRST, typename I>
+__global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs<I> a, ZeroPart zeros) {
     __shared__ uint32_t cnt[4][1 << kSortBits];  // per wave: count, then where its entries of the digit go
     __shared__ uint32_t wsum[4];
-    if (blockIdx.x >= a.tiles) return store_zeros(zeros, blockIdx.x - a.tiles);
+    if (blockIdx.x >= a.tiles) return store_zeros<256>(zeros, blockIdx.x - a.tiles, gridDim.x - a.tiles);
     if (*a.ascend) return;
     const uint32_t bins = 1u << a.bits;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
@@ -245,34 +349,20 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs a, Zer
     }
     for (uint32_t b = tid; b < 4 * bins; b += 256) cnt[b >> a.bits][b & (bins - 1)] = 0;
     __syncthreads();
-    // the lanes of this wave whose digit equals mine; the first of them adds their number
     uint64_t same[kSortRounds];
     uint32_t old[kSortRounds];
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
         const bool on = base + r * 64 + lane < a.n;
         const uint32_t d = (e[r].x >> a.shift) & (bins - 1);
-        uint64_t s = __ballot(on);
-        if (!on) s = ~s;
-#pragma unroll
-        for (int k = 0; k < kSortBits; ++k)
-            if (k < a.bits) {
-                const uint64_t m = __ballot((d >> k) & 1);
-                s &= (d >> k) & 1 ? m : ~m;
-            }
-        same[r] = s;
+        same[r] = match<kSortBits>(d, on, a.bits);
         old[r] = 0;
-        if (on && (s & ((1ull << lane) - 1)) == 0) old[r] = atomicAdd(&cnt[w][d], (uint32_t)__popcll(s));
+        if (on && (same[r] & below(lane)) == 0) old[r] = atomicAdd(&cnt[w][d], (uint32_t)__popcll(same[r]));
     }
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r)  // the entry's place among the wave's entries of its digit
-        old[r] = __shfl(old[r], __ffsll((unsigned long long)same[r]) - 1) + __popcll(same[r] & ((1ull << lane) - 1));
-    uint32_t inc = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(inc, d);
-        if (lane >= d) inc += o;
-    }
+    for (int r = 0; r < kSortRounds; ++r)
+        old[r] = __shfl(old[r], __ffsll((unsigned long long)same[r]) - 1) + __popcll(same[r] & below(lane));
+    const uint32_t inc = wave_scan(sum, lane);
     if (lane == 63) wsum[w] = inc;
     __syncthreads();
     uint32_t at = inc - sum;
@@ -299,47 +389,40 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs a, Zer
 
 // --------------------------------------------------------------------------------------- sums
 // A subgroup of `lanes` lanes holds VEC columns per lane; columns beyond lanes * VEC: grid.y.
+template <typename I>
 struct SumArgs {
     uint32_t n, V;
     int64_t D;
-    RowIds ids;
+    RowIds<I> ids;
     const uint2* list;       // sorted (id, i)
     const uint32_t* ascend;  // not null and set: the ids ascend by themselves, no list was made
     const void* g;
     int64_t gstride;
     void* dw;
     int64_t dwstride;
-    int dwtype, accumulate;
+    int accumulate;
     float scale;
     int lanes;           // lanes per subgroup, a power of two
+    int run;             // entries per subgroup
     uint32_t blocks;     // workgroups over the entries
     float *head, *tail;  // [blocks][D]: the sums of a workgroup's runs that began before it / go on after it
     uint32_t rows;       // table form: entries per workgroup; few entries: rows per zeroing workgroup
     uint8_t* named;      // table form: [blocks][V]
 };
 
-template <int VEC>
-__device__ __forceinline__ void put_row(const SumArgs& a, uint32_t v, int64_t col, const float* acc) {
-    const int64_t at = (int64_t)v * a.dwstride + col;
-    auto put = [&](auto* p) {
-        using OT = typename std::remove_pointer<decltype(p)>::type;
-        Vec<OT, VEC> o;
-        if (a.accumulate) {
-            o = load_vec<OT, VEC>(p);
+template <typename OT, int VEC, typename I>
+__device__ __forceinline__ void put_row(const SumArgs<I>& a, uint32_t v, int64_t col, const float* acc) {
+    OT* p = static_cast<OT*>(a.dw) + (int64_t)v * a.dwstride + col;
+    Vec<OT, VEC> o;
+    if (a.accumulate) {
+        o = load_vec<OT, VEC>(p);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) o.v[k] = (OT)((float)o.v[k] + acc[k] * a.scale);
-        } else {
+        for (int k = 0; k < VEC; ++k) o.v[k] = (OT)((float)o.v[k] + acc[k] * a.scale);
+    } else {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) o.v[k] = (OT)(acc[k] * a.scale);
-        }
-        store_vec<OT, VEC>(p, o);
-    };
-    if (a.dwtype == HGSR_F32)
-        put(static_cast<float*>(a.dw) + at);
-    else if (a.dwtype == HGSR_F16)
-        put(static_cast<f16_t*>(a.dw) + at);
-    else
-        put(static_cast<bf16_t*>(a.dw) + at);
+        for (int k = 0; k < VEC; ++k) o.v[k] = (OT)(acc[k] * a.scale);
+    }
+    store_vec<OT, VEC>(p, o);
 }
 
 template <typename T, int VEC>
@@ -348,14 +431,31 @@ __device__ __forceinline__ void add_vec(float* acc, const Vec<T, VEC>& x) {
     for (int c = 0; c < VEC; ++c) acc[c] += (float)x.v[c];
 }
 
+// acc of the first `live` subgroups (at least 1; the others hold nothing) summed into subgroup 0's, in
+// a fixed tree; every thread of the workgroup calls it
+template <int VEC>
+__device__ __forceinline__ void sum_subgroups(Vec<float, VEC>* part, float* acc, int lanes, int live) {
+    const int tid = threadIdx.x, s = tid / lanes;
+    int h = 1;
+    while (h < live) h <<= 1;
+    for (h >>= 1; h > 0; h >>= 1) {
+        if (s >= h && s < 2 * h) {
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) part[tid].v[c] = acc[c];
+        }
+        __syncthreads();
+        if (s < h) add_vec<float, VEC>(acc, part[tid + h * lanes]);
+    }
+}
+
 // ---- few entries: one launch, a workgroup per entry.  The first of the entries that name a row
 // sums them all (each subgroup every NS-th of them, joined through LDS); other workgroups store the
 // zeros of the rows that no id names.
 constexpr int kFewMost = 256;
 constexpr int kFewRows = 1024;  // rows per zeroing workgroup, at most
 
-template <typename GT, int VEC>
-__global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs a) {
+template <typename GT, typename OT, typename I, int VEC>
+__global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
     __shared__ Vec<float, VEC> part[256];
     __shared__ uint32_t match[kFewMost];
     __shared__ uint32_t count[4], first[4];
@@ -373,7 +473,7 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs a) {
         __syncthreads();
         const float z[VEC] = {};
         for (uint32_t k = s; k < a.rows && r0 + k < a.V; k += NS)
-            if (on && !named[k]) put_row<VEC>(a, r0 + k, col, z);
+            if (on && !named[k]) put_row<OT, VEC>(a, r0 + k, col, z);
         return;
     }
     const uint32_t v = a.ids.get(blockIdx.x, a.V);
@@ -406,22 +506,16 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs a) {
                 if (j + u * NS < m) add_vec<GT, VEC>(acc, x[u]);
         }
     }
-    Vec<float, VEC> o;
-#pragma unroll
-    for (int c = 0; c < VEC; ++c) o.v[c] = acc[c];
-    part[tid] = o;
-    __syncthreads();
-    if (s || !on) return;
-    for (uint32_t q = 1; q < (uint32_t)NS && q < m; ++q) add_vec<float, VEC>(acc, part[q * L + ln]);
-    put_row<VEC>(a, v, col, acc);
+    sum_subgroups<VEC>(part, acc, L, m < (uint32_t)NS ? (int)m : NS);
+    if (s == 0 && on) put_row<OT, VEC>(a, v, col, acc);
 }
 
 // ---- few rows: no sort.  Every subgroup keeps a table of sums in LDS, its own, so a workgroup's
 // entries are read once and in order; the subgroups' and then the workgroups' tables are added.
 constexpr int kTableMost = 64;  // V * VEC: 64 KB of LDS, two workgroups per compute unit
 
-template <typename GT, int VEC>
-__global__ __launch_bounds__(256) void embed_table_kernel(const SumArgs a) {
+template <typename GT, typename I, int VEC>
+__global__ __launch_bounds__(256) void embed_table_kernel(const SumArgs<I> a) {
     extern __shared__ __align__(16) char smem[];
     Vec<float, VEC>* tab = reinterpret_cast<Vec<float, VEC>*>(smem);  // [V][256]
     __shared__ uint8_t named[kTableMost];
@@ -434,7 +528,7 @@ __global__ __launch_bounds__(256) void embed_table_kernel(const SumArgs a) {
     for (uint32_t v = 0; v < a.V; ++v) tab[v * 256 + tid] = zero;
     if (tid < kTableMost) named[tid] = 0;
     __syncthreads();
-    const GT* g = static_cast<const GT*>(a.g) + col;
+    const GT* g = static_cast<const GT*>(a.g) + (on ? col : 0);
     const uint64_t i1 = min((uint64_t)a.n, ((uint64_t)blockIdx.x + 1) * a.rows);
     for (uint64_t i0 = (uint64_t)blockIdx.x * a.rows + s; i0 < i1; i0 += 8 * NS) {
         uint32_t id[8];
@@ -442,8 +536,10 @@ __global__ __launch_bounds__(256) void embed_table_kernel(const SumArgs a) {
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int64_t i = i0 + u * NS;
-            id[u] = i < (int64_t)i1 ? a.ids.get(i, a.V) : a.V;
-            if (on && i < (int64_t)i1) x[u] = load_vec<GT, VEC>(g + i * a.gstride);
+            const int64_t j = i < (int64_t)i1 ? i : i1 - 1;
+            id[u] = a.ids.get(j, a.V);
+            if (j != i) id[u] = a.V;
+            x[u] = load_vec<GT, VEC>(g + j * a.gstride);
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u)
@@ -467,10 +563,10 @@ __global__ __launch_bounds__(256) void embed_table_kernel(const SumArgs a) {
     if (blockIdx.y == 0 && (uint32_t)tid < a.V) a.named[(int64_t)blockIdx.x * a.V + tid] = named[tid];
 }
 
-template <int VEC>
-__global__ __launch_bounds__(256) void embed_table_join_kernel(const SumArgs a) {
-    __shared__ Vec<float, VEC> part[256];
-    const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
+template <typename OT, typename I, int VEC>
+__global__ __launch_bounds__(1024) void embed_table_join_kernel(const SumArgs<I> a) {
+    __shared__ Vec<float, VEC> part[1024];
+    const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 1024 / L;
     const uint32_t v = blockIdx.x, share = (a.blocks + NS - 1) / NS;
     const int64_t col = ((int64_t)blockIdx.y * L + ln) * VEC;
     const bool on = col < a.D;
@@ -486,64 +582,64 @@ __global__ __launch_bounds__(256) void embed_table_join_kernel(const SumArgs a) 
             for (int c = 0; c < VEC; ++c) acc[c] += p[c];
         }
     }
-    Vec<float, VEC> o;
-#pragma unroll
-    for (int c = 0; c < VEC; ++c) o.v[c] = acc[c];
-    part[tid] = o;
     hit = __syncthreads_or(hit);
-    if (s || !on || (a.accumulate && !hit)) return;
-    for (int q = 1; q < NS && (uint32_t)q * share < a.blocks; ++q) add_vec<float, VEC>(acc, part[q * L + ln]);
-    put_row<VEC>(a, v, col, acc);
+    sum_subgroups<VEC>(part, acc, L, NS);
+    if (s == 0 && on && (hit || !a.accumulate)) put_row<OT, VEC>(a, v, col, acc);
 }
 
-// ---- the general form: every subgroup walks kSumRun consecutive entries of the sorted list, and a
-// workgroup's 256 / lanes subgroups take consecutive pieces.
+// ---- the general form: every subgroup walks `run` consecutive entries of the sorted list, and a
+// workgroup's 256 / lanes subgroups take consecutive pieces.  run: 16, or 8 where 16 would leave
+// compute units without a workgroup.
 constexpr int kSumRun = 16;
 
-__device__ __forceinline__ uint32_t sorted_id(const SumArgs& a, bool asc, uint32_t i) {
+template <typename I>
+__device__ __forceinline__ uint32_t sorted_id(const SumArgs<I>& a, bool asc, uint32_t i) {
     return asc ? a.ids.get(i, a.V) : a.list[i].x;
 }
 
-template <typename GT, int VEC>
-__global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
+template <typename GT, typename OT, typename I, int VEC>
+__global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs<I> a) {
     extern __shared__ uint32_t key[];         // [1 + E + 1]: the entry before, the workgroup's, the one after
     __shared__ Vec<float, VEC> part[2][256];  // [0]: run that began before the subgroup, [1]: goes on after it
     __shared__ int state[256];                // 1: has a part[0], 2: which goes on after it, 4: has a part[1]
     const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
-    const uint32_t E = NS * kSumRun, block = xcd_remap(blockIdx.x, gridDim.x);
+    const uint32_t E = NS * a.run, block = xcd_remap(blockIdx.x, gridDim.x);
     uint32_t* pos = key + E + 2;
     const int64_t col = ((int64_t)blockIdx.y * L + ln) * VEC;
     const bool on = col < a.D, asc = a.ascend && *a.ascend;
     constexpr uint32_t NONE = ~0u;
     const uint32_t i0 = block * E;
-    for (uint32_t k = tid; k < E; k += 256) {
-        const uint32_t i = i0 + k;
+#pragma unroll
+    for (uint32_t q = 0; q < kSumRun * 64 / 256; ++q) {  // E <= 64 * kSumRun
+        const uint32_t k = q * 256 + tid, i = i0 + k;
+        if (k >= E) break;
         uint2 e = make_uint2(NONE, 0);
         if (i < a.n) e = asc ? make_uint2(a.ids.get(i, a.V), i) : a.list[i];
         key[1 + k] = e.x;
-        pos[k] = e.y;
+        pos[k] = e.x < a.V ? e.y : 0;  // of entries without a row, row 0 of g is read and not used
     }
     if (tid == 0) key[0] = i0 ? sorted_id(a, asc, i0 - 1) : NONE;
     if (tid == 64) key[1 + E] = i0 + E < a.n ? sorted_id(a, asc, i0 + E) : NONE;
     __syncthreads();
-    const GT* g = static_cast<const GT*>(a.g) + col;
-    const int e0 = s * kSumRun;
+    const GT* g = static_cast<const GT*>(a.g) + (on ? col : 0);
+    const int e0 = s * a.run;
     float acc[VEC] = {};
     bool head = key[e0] == key[1 + e0];  // the first run began before this subgroup
     int st = 0;
-    for (int k0 = 0; k0 < kSumRun; k0 += 8) {
+    for (int k0 = 0; k0 < a.run; k0 += 8) {
         Vec<GT, VEC> x[8];
+        uint32_t id[9];
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (on && key[1 + e0 + k0 + u] < a.V) x[u] = load_vec<GT, VEC>(g + (int64_t)pos[e0 + k0 + u] * a.gstride);
+        for (int u = 0; u < 9; ++u) id[u] = key[1 + e0 + k0 + u];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = load_vec<GT, VEC>(g + (int64_t)pos[e0 + k0 + u] * a.gstride);
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const int k = e0 + k0 + u;
-            const uint32_t v = key[1 + k];
+            const uint32_t v = id[u];
             if (v >= a.V) continue;  // no row: nothing of it is summed
             add_vec<GT, VEC>(acc, x[u]);
-            const bool goes_on = key[2 + k] == v;
-            if (goes_on && k0 + u < kSumRun - 1) continue;
+            const bool goes_on = id[u + 1] == v;
+            if (goes_on && k0 + u < a.run - 1) continue;
             if (head || goes_on) {
                 Vec<float, VEC> o;
 #pragma unroll
@@ -551,7 +647,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
                 part[head ? 0 : 1][tid] = o;
                 st |= head ? (goes_on ? 3 : 1) : 4;
             } else if (on) {
-                put_row<VEC>(a, v, col, acc);
+                put_row<OT, VEC>(a, v, col, acc);
             }
             head = false;
 #pragma unroll
@@ -577,7 +673,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
         if (open)
             keep(a.tail);
         else
-            put_row<VEC>(a, key[e0 + kSumRun], col, acc);
+            put_row<OT, VEC>(a, key[e0 + a.run], col, acc);
     }
     if (s == 0 && (st & 1)) {  // the run that an earlier workgroup began
 #pragma unroll
@@ -589,13 +685,13 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs a) {
 
 // One workgroup per workgroup of the sums: if a run begins in it and goes on, its tail and the
 // heads of the workgroups it reaches into, each subgroup a consecutive share, joined through LDS.
-template <int VEC>
-__global__ __launch_bounds__(256) void embed_join_kernel(const SumArgs a) {
+template <typename OT, typename I, int VEC>
+__global__ __launch_bounds__(256) void embed_join_kernel(const SumArgs<I> a) {
     __shared__ Vec<float, VEC> part[256];
     __shared__ uint32_t s_last;
     const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
     const bool asc = a.ascend && *a.ascend;
-    const uint32_t E = NS * kSumRun, b = blockIdx.x, i0 = b * E, i1 = i0 + E;
+    const uint32_t E = NS * a.run, b = blockIdx.x, i0 = b * E, i1 = i0 + E;
     if (i1 >= a.n) return;
     const uint32_t v = sorted_id(a, asc, i1);
     if (v >= a.V || sorted_id(a, asc, i1 - 1) != v || (b && sorted_id(a, asc, i0 - 1) == v)) return;
@@ -624,34 +720,30 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const SumArgs a) {
             for (int c = 0; c < VEC; ++c) acc[c] += p[c];
         }
     }
-    Vec<float, VEC> o;
+    if (on && s == 0) {
+        const float* p = a.tail + (int64_t)b * a.D + col;
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) o.v[c] = acc[c];
-    part[tid] = o;
-    __syncthreads();
-    if (s || !on) return;
-    const float* p = a.tail + (int64_t)b * a.D + col;
-#pragma unroll
-    for (int c = 0; c < VEC; ++c) acc[c] += p[c];
-    for (int q = 1; q < NS && (uint32_t)q * share < m; ++q) add_vec<float, VEC>(acc, part[q * L + ln]);
-    put_row<VEC>(a, v, col, acc);
+        for (int c = 0; c < VEC; ++c) acc[c] += p[c];
+    }
+    sum_subgroups<VEC>(part, acc, L, m < (uint32_t)NS ? (int)m : NS);
+    if (s == 0 && on) put_row<OT, VEC>(a, v, col, acc);
 }
 
 // ---------------------------------------------------------------------------------- launches
 
-enum BwdForm { kFew, kTable, kRank, kRadix };
+enum BwdForm { kFew, kTable, kBucket, kRadix };
 
 struct BwdPlan {
     BwdForm form;
-    int lanes, passes, bits;
-    uint32_t tiles, blocks, slabs, rows;
+    int lanes, run, shift, passes, bits;
+    uint32_t buckets, tiles, blocks, slabs, rows;
     size_t list_a, list_b, hist, total, ascend, head, tail, named, bytes;
 };
 
 static BwdPlan bwd_plan(int64_t V, int64_t n, int64_t D, int vec) {
     BwdPlan p{};
     const int64_t per_row = (D + vec - 1) / vec;
-    p.lanes = 1;
+    p.lanes = 4;  // at least: 64 subgroups per workgroup at most
     while (p.lanes < 64 && p.lanes < per_row) p.lanes <<= 1;
     const int64_t NS = 256 / p.lanes;
     p.slabs = (uint32_t)((per_row + p.lanes - 1) / p.lanes);
@@ -661,7 +753,7 @@ static BwdPlan bwd_plan(int64_t V, int64_t n, int64_t D, int vec) {
         o += align256(b);
         return at;
     };
-    p.form = n <= kFewMost ? kFew : V * vec <= kTableMost ? kTable : n <= kRankMost ? kRank : kRadix;
+    p.form = n <= kFewMost ? kFew : V * vec <= kTableMost ? kTable : n <= kBucketMost ? kBucket : kRadix;
     if (p.form == kTable) {
         int64_t blocks = 512 / p.slabs;  // two per compute unit
         if (blocks < 1) blocks = 1;
@@ -671,15 +763,22 @@ static BwdPlan bwd_plan(int64_t V, int64_t n, int64_t D, int vec) {
         p.head = take((size_t)p.blocks * V * D * 4);
         p.named = take((size_t)p.blocks * V);
     } else if (p.form != kFew) {
-        p.blocks = (uint32_t)((n + NS * kSumRun - 1) / (NS * kSumRun));
+        p.run = (n / (NS * kSumRun) + 1) * p.slabs < 256 ? 8 : kSumRun;
+        p.blocks = (uint32_t)((n + NS * p.run - 1) / (NS * p.run));
         p.list_a = take((size_t)n * 8);
         p.head = take((size_t)p.blocks * D * 4);
         p.tail = take((size_t)p.blocks * D * 4);
+        int key_bits = 1;
+        while ((V >> key_bits) != 0) ++key_bits;  // ids 0 .. V (V: no row)
+        if (p.form == kBucket) {
+            p.shift = key_bits > kBucketLog ? key_bits - kBucketLog : 0;
+            p.buckets = (uint32_t)(V >> p.shift) + 1;
+            key_bits = p.shift;
+        }
+        const int most = p.form == kBucket ? kBucketBits : kSortBits;
+        p.passes = (key_bits + most - 1) / most;
+        p.bits = p.passes ? (key_bits + p.passes - 1) / p.passes : 0;
         if (p.form == kRadix) {
-            int key_bits = 1;
-            while ((V >> key_bits) != 0) ++key_bits;  // ids 0 .. V (V: no row)
-            p.passes = (key_bits + kSortBits - 1) / kSortBits;
-            p.bits = (key_bits + p.passes - 1) / p.passes;
             p.tiles = (uint32_t)((n + kSortTile - 1) / kSortTile);
             p.list_b = take((size_t)n * 8);
             p.hist = take(((size_t)p.tiles << p.bits) * 4);
@@ -727,17 +826,18 @@ struct ZeroPlan {
 };
 
 // sorts the ids: a.list, or a.ascend where they may turn out to be sorted
-static void launch_sort(const BwdPlan& p, char* w, SumArgs& a, ZeroPlan zeros, hipStream_t s) {
+template <typename I>
+static void launch_sort(const BwdPlan& p, char* w, SumArgs<I>& a, ZeroPlan zeros, hipStream_t s) {
     uint2 *la = reinterpret_cast<uint2*>(w + p.list_a), *lb = reinterpret_cast<uint2*>(w + p.list_b);
     uint32_t zb;
-    if (p.form == kRank) {
-        const uint32_t blocks = (a.n + 4 * kRankOwn - 1) / (4 * kRankOwn);
+    if (p.form == kBucket) {
         const ZeroPart z = zeros.take(zb);
-        hipLaunchKernelGGL(sort_rank_kernel, dim3(blocks + zb), dim3(256), 0, s, a.n, a.ids, a.V, la, blocks, z);
+        hipLaunchKernelGGL((sort_bucket_kernel<I>), dim3(p.buckets + zb), dim3(1024), 0, s, a.n, a.ids, a.V, p.shift,
+                           p.passes, p.bits, la, p.buckets, z);
         a.list = la;
         return;
     }
-    SortArgs t{};
+    SortArgs<I> t{};
     t.n = a.n;
     t.V = a.V;
     t.ids = a.ids;
@@ -753,82 +853,128 @@ static void launch_sort(const BwdPlan& p, char* w, SumArgs& a, ZeroPlan zeros, h
         t.shift = pass * p.bits;
         const ZeroPart z0 = zeros.take(zb);
         if (pass == 0) {
-            hipLaunchKernelGGL((sort_count_kernel<true>), dim3(p.tiles + zb), dim3(256), 0, s, t, z0);
-            hipLaunchKernelGGL((sort_scan_kernel<true>), dim3(scan_blocks + 1), dim3(1024), 0, s, t);
+            hipLaunchKernelGGL((sort_count_kernel<true, I>), dim3(p.tiles + zb), dim3(256), 0, s, t, z0);
+            hipLaunchKernelGGL((sort_scan_kernel<true, I>), dim3(scan_blocks + 1), dim3(1024), 0, s, t);
         } else {
-            hipLaunchKernelGGL((sort_count_kernel<false>), dim3(p.tiles + zb), dim3(256), 0, s, t, z0);
-            hipLaunchKernelGGL((sort_scan_kernel<false>), dim3(scan_blocks), dim3(1024), 0, s, t);
+            hipLaunchKernelGGL((sort_count_kernel<false, I>), dim3(p.tiles + zb), dim3(256), 0, s, t, z0);
+            hipLaunchKernelGGL((sort_scan_kernel<false, I>), dim3(scan_blocks), dim3(1024), 0, s, t);
         }
         const ZeroPart z1 = zeros.take(zb);
         if (pass == 0)
-            hipLaunchKernelGGL((sort_scatter_kernel<true>), dim3(p.tiles + zb), dim3(256), 0, s, t, z1);
+            hipLaunchKernelGGL((sort_scatter_kernel<true, I>), dim3(p.tiles + zb), dim3(256), 0, s, t, z1);
         else
-            hipLaunchKernelGGL((sort_scatter_kernel<false>), dim3(p.tiles + zb), dim3(256), 0, s, t, z1);
+            hipLaunchKernelGGL((sort_scatter_kernel<false, I>), dim3(p.tiles + zb), dim3(256), 0, s, t, z1);
     }
     a.list = t.out;
     a.ascend = t.ascend;
 }
 
-template <typename GT, int VEC>
-static void launch_sums(const BwdPlan& p, const SumArgs& a, uint32_t zero_blocks, hipStream_t s) {
+template <typename GT, typename OT, int VEC, typename I>
+static void launch_sums(const BwdPlan& p, const SumArgs<I>& a, uint32_t zero_blocks, hipStream_t s) {
     const dim3 block(256);
     switch (p.form) {
         case kFew:
-            hipLaunchKernelGGL((embed_few_kernel<GT, VEC>), dim3(a.n + zero_blocks, p.slabs), block, 0, s, a);
+            hipLaunchKernelGGL((embed_few_kernel<GT, OT, I, VEC>), dim3(a.n + zero_blocks, p.slabs), block, 0, s, a);
             break;
         case kTable:
-            hipLaunchKernelGGL((embed_table_kernel<GT, VEC>), dim3(a.blocks, p.slabs), block,
+            hipLaunchKernelGGL((embed_table_kernel<GT, I, VEC>), dim3(a.blocks, p.slabs), block,
                                (size_t)a.V * 256 * VEC * sizeof(float), s, a);
-            hipLaunchKernelGGL((embed_table_join_kernel<VEC>), dim3(a.V, p.slabs), block, 0, s, a);
+            hipLaunchKernelGGL((embed_table_join_kernel<OT, I, VEC>), dim3(a.V, p.slabs), dim3(1024), 0, s,
+                               a);
             break;
         default:
-            hipLaunchKernelGGL((embed_sum_kernel<GT, VEC>), dim3(a.blocks, p.slabs), block,
-                               (2 * (256 / a.lanes) * kSumRun + 2) * sizeof(uint32_t), s, a);
+            hipLaunchKernelGGL((embed_sum_kernel<GT, OT, I, VEC>), dim3(a.blocks, p.slabs), block,
+                               (2 * (256 / a.lanes) * a.run + 2) * sizeof(uint32_t), s, a);
             if (a.blocks > 1)
-                hipLaunchKernelGGL((embed_join_kernel<VEC>), dim3(a.blocks, p.slabs), block, 0, s, a);
+                hipLaunchKernelGGL((embed_join_kernel<OT, I, VEC>), dim3(a.blocks, p.slabs), block, 0, s, a);
     }
 }
 
-template <typename GT>
-static void launch_sums(int vec, const BwdPlan& p, const SumArgs& a, uint32_t zero_blocks, hipStream_t s) {
+template <typename GT, typename OT, typename I>
+static void launch_sums(int vec, const BwdPlan& p, const SumArgs<I>& a, uint32_t zero_blocks, hipStream_t s) {
     switch (vec) {
-        case 8: return launch_sums<GT, 8>(p, a, zero_blocks, s);
-        case 4: return launch_sums<GT, 4>(p, a, zero_blocks, s);
-        case 2: return launch_sums<GT, 2>(p, a, zero_blocks, s);
-        default: return launch_sums<GT, 1>(p, a, zero_blocks, s);
+        case 8: return launch_sums<GT, OT, sizeof(GT) == 4 ? 4 : 8>(p, a, zero_blocks, s);
+        case 4: return launch_sums<GT, OT, 4>(p, a, zero_blocks, s);
+        case 2: return launch_sums<GT, OT, 2>(p, a, zero_blocks, s);
+        default: return launch_sums<GT, OT, 1>(p, a, zero_blocks, s);
     }
 }
 
-template <typename WT, typename OT, int VEC>
-static void launch_fwd(int64_t V, int64_t n, int64_t D, const void* w, int64_t wstride, RowIds ids, float scale,
-                       void* out, hipStream_t s) {
-    const uint32_t per_row = (uint32_t)(D / VEC);
+template <typename GT, typename I>
+static void launch_sums(int dwtype, int vec, const BwdPlan& p, const SumArgs<I>& a, uint32_t zero_blocks,
+                        hipStream_t s) {
+    if (dwtype == HGSR_F32) return launch_sums<GT, float>(vec, p, a, zero_blocks, s);
+    if (dwtype == HGSR_F16) return launch_sums<GT, f16_t>(vec, p, a, zero_blocks, s);
+    return launch_sums<GT, bf16_t>(vec, p, a, zero_blocks, s);
+}
+
+template <typename I>
+static int launch_bwd(const BwdPlan& p, char* w, SumArgs<I> a, const void* ids, int64_t ids_stride, int gtype,
+                      int dwtype, int vec, hipStream_t s) {
+    a.ids = RowIds<I>{static_cast<const I*>(ids), ids_stride};
+    KernelTimer kt("embed_bwd", s);
+    uint32_t zero_blocks = 0;
+    const size_t dw_bytes = (size_t)a.V * a.D * elem_size(dwtype);
+    if (p.form == kFew && !a.accumulate) {  // about 32 KB of zeros per workgroup
+        const int64_t rows = 32768 / ((int64_t)p.lanes * vec * elem_size(dwtype));
+        a.rows = (uint32_t)(rows < 1 ? 1 : rows > kFewRows ? kFewRows : rows);
+        zero_blocks = (a.V + a.rows - 1) / a.rows;
+    } else if (p.form == kBucket || p.form == kRadix) {
+        ZeroPlan zeros;
+        if (!a.accumulate) zeros = ZeroPlan(a.dw, dw_bytes, p.form == kBucket ? 1 : 2 * p.passes);
+        launch_sort(p, w, a, zeros, s);
+    }
+    if (gtype == HGSR_F32)
+        launch_sums<float>(dwtype, vec, p, a, zero_blocks, s);
+    else if (gtype == HGSR_F16)
+        launch_sums<f16_t>(dwtype, vec, p, a, zero_blocks, s);
+    else
+        launch_sums<bf16_t>(dwtype, vec, p, a, zero_blocks, s);
+    return check_launch("embed_bwd");
+}
+
+struct FwdArgs {
+    int64_t V, n, D, wstride, ids_stride;
+    const void *w, *ids;
+    int ids64;
+    float scale;
+    void* out;
+};
+
+template <typename WT, typename OT, typename I, int VEC>
+static void launch_fwd(const FwdArgs& a, hipStream_t s) {
+    const uint32_t per_row = (uint32_t)(a.D / VEC);
+    const RowIds<I> ids{static_cast<const I*>(a.ids), a.ids_stride};
     const int64_t most = ((int64_t)1 << 30) / per_row;  // rows per launch: at most 2^30 pieces
-    for (int64_t r0 = 0; r0 < n; r0 += most) {
-        const uint32_t chunks = (uint32_t)((n - r0 < most ? n - r0 : most) * per_row);
-        hipLaunchKernelGGL((embed_fwd_kernel<WT, OT, VEC>), dim3((chunks + 256 * kFwdPer - 1) / (256 * kFwdPer)), dim3(256), 0, s, chunks,
-                           fast_div(per_row), (uint32_t)V, static_cast<const WT*>(w), wstride, ids, r0, scale,
-                           static_cast<OT*>(out));
+    for (int64_t r0 = 0; r0 < a.n; r0 += most) {
+        const uint32_t chunks = (uint32_t)((a.n - r0 < most ? a.n - r0 : most) * per_row);
+        hipLaunchKernelGGL((embed_fwd_kernel<WT, OT, I, VEC>), dim3((chunks + 255) / 256), dim3(256), 0, s, chunks,
+                           fast_div(per_row), (uint32_t)a.V, static_cast<const WT*>(a.w),
+                           a.wstride, ids, r0, a.scale, static_cast<OT*>(a.out),
+                           stream_out(a.n * a.D * (int64_t)sizeof(OT)));
+    }
+}
+
+template <typename WT, typename OT, typename I>
+static void launch_fwd(int vec, const FwdArgs& a, hipStream_t s) {
+    switch (vec) {
+        case 8: return launch_fwd<WT, OT, I, sizeof(WT) + sizeof(OT) == 4 ? 8 : 4>(a, s);
+        case 4: return launch_fwd<WT, OT, I, 4>(a, s);
+        case 2: return launch_fwd<WT, OT, I, 2>(a, s);
+        default: return launch_fwd<WT, OT, I, 1>(a, s);
     }
 }
 
 template <typename WT, typename OT>
-static void launch_fwd(int vec, int64_t V, int64_t n, int64_t D, const void* w, int64_t wstride, RowIds ids,
-                       float scale, void* out, hipStream_t s) {
-    switch (vec) {
-        case 8: return launch_fwd<WT, OT, 8>(V, n, D, w, wstride, ids, scale, out, s);
-        case 4: return launch_fwd<WT, OT, 4>(V, n, D, w, wstride, ids, scale, out, s);
-        case 2: return launch_fwd<WT, OT, 2>(V, n, D, w, wstride, ids, scale, out, s);
-        default: return launch_fwd<WT, OT, 1>(V, n, D, w, wstride, ids, scale, out, s);
-    }
+static void launch_fwd(int vec, const FwdArgs& a, hipStream_t s) {
+    return a.ids64 ? launch_fwd<WT, OT, int64_t>(vec, a, s) : launch_fwd<WT, OT, int32_t>(vec, a, s);
 }
 
 template <typename WT>
-static void launch_fwd(int otype, int vec, int64_t V, int64_t n, int64_t D, const void* w, int64_t wstride, RowIds ids,
-                       float scale, void* out, hipStream_t s) {
-    if (otype == HGSR_F32) return launch_fwd<WT, float>(vec, V, n, D, w, wstride, ids, scale, out, s);
-    if (otype == HGSR_F16) return launch_fwd<WT, f16_t>(vec, V, n, D, w, wstride, ids, scale, out, s);
-    return launch_fwd<WT, bf16_t>(vec, V, n, D, w, wstride, ids, scale, out, s);
+static void launch_fwd(int otype, int vec, const FwdArgs& a, hipStream_t s) {
+    if (otype == HGSR_F32) return launch_fwd<WT, float>(vec, a, s);
+    if (otype == HGSR_F16) return launch_fwd<WT, f16_t>(vec, a, s);
+    return launch_fwd<WT, bf16_t>(vec, a, s);
 }
 
 }  // namespace hgsr
@@ -854,16 +1000,16 @@ extern "C" int hgsr_embed_fwd(int64_t V, int64_t n, int64_t D, const void* weigh
     int vec = vec_width(most, D, wstride, weight, elem_size(wtype));
     const int vo = vec_width(most, D, D, out, elem_size(otype));
     if (vo < vec) vec = vo;
-    const RowIds id{ids, ids_stride, ids64};
+    const FwdArgs a{V, n, D, wstride, ids_stride, weight, ids, ids64, scale, out};
     hipStream_t s = as_stream(stream);
     {
         KernelTimer kt("embed_fwd", s);
         if (wtype == HGSR_F32)
-            launch_fwd<float>(otype, vec, V, n, D, weight, wstride, id, scale, out, s);
+            launch_fwd<float>(otype, vec, a, s);
         else if (wtype == HGSR_F16)
-            launch_fwd<f16_t>(otype, vec, V, n, D, weight, wstride, id, scale, out, s);
+            launch_fwd<f16_t>(otype, vec, a, s);
         else
-            launch_fwd<bf16_t>(otype, vec, V, n, D, weight, wstride, id, scale, out, s);
+            launch_fwd<bf16_t>(otype, vec, a, s);
     }
     return check_launch("embed_fwd");
 }
@@ -890,18 +1036,6 @@ extern "C" int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, in
     hipStream_t s = as_stream(stream);
     const size_t dw_bytes = (size_t)V * D * elem_size(dwtype);
     HGSR_REQUIRE(dw_bytes / (kZeroUnits * 16) < (1ull << 30), "embed_bwd: table too large");
-    SumArgs a{};
-    a.n = (uint32_t)n;
-    a.V = (uint32_t)V;
-    a.D = D;
-    a.ids = RowIds{ids, ids_stride, ids64};
-    a.g = g;
-    a.gstride = gstride;
-    a.dw = dw;
-    a.dwstride = dwstride;
-    a.dwtype = dwtype;
-    a.accumulate = accumulate != 0;
-    a.scale = scale;
     if (n == 0) {
         if (!accumulate) {
             uint32_t zb;
@@ -922,28 +1056,25 @@ extern "C" int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, in
         return HGSR_EWORKSPACE;
     }
     char* w = static_cast<char*>(ws);
-    a.lanes = p.lanes;
-    a.blocks = p.blocks;
-    a.rows = p.rows;
-    a.head = reinterpret_cast<float*>(w + p.head);
-    a.tail = reinterpret_cast<float*>(w + p.tail);
-    a.named = reinterpret_cast<uint8_t*>(w + p.named);
-    KernelTimer kt("embed_bwd", s);
-    uint32_t zero_blocks = 0;
-    if (p.form == kFew && !accumulate) {  // about 32 KB of zeros per workgroup
-        const int64_t rows = 32768 / ((int64_t)p.lanes * vec * elem_size(dwtype));
-        a.rows = (uint32_t)(rows < 1 ? 1 : rows > kFewRows ? kFewRows : rows);
-        zero_blocks = (uint32_t)((V + a.rows - 1) / a.rows);
-    } else if (p.form == kRank || p.form == kRadix) {
-        ZeroPlan zeros;
-        if (!accumulate) zeros = ZeroPlan(dw, dw_bytes, p.form == kRank ? 1 : 2 * p.passes);
-        launch_sort(p, w, a, zeros, s);
-    }
-    if (gtype == HGSR_F32)
-        launch_sums<float>(vec, p, a, zero_blocks, s);
-    else if (gtype == HGSR_F16)
-        launch_sums<f16_t>(vec, p, a, zero_blocks, s);
-    else
-        launch_sums<bf16_t>(vec, p, a, zero_blocks, s);
-    return check_launch("embed_bwd");
+    auto run = [&](auto none) {
+        SumArgs<decltype(none)> a{};
+        a.n = (uint32_t)n;
+        a.V = (uint32_t)V;
+        a.D = D;
+        a.g = g;
+        a.gstride = gstride;
+        a.dw = dw;
+        a.dwstride = dwstride;
+        a.accumulate = accumulate != 0;
+        a.scale = scale;
+        a.lanes = p.lanes;
+        a.run = p.run;
+        a.blocks = p.blocks;
+        a.rows = p.rows;
+        a.head = reinterpret_cast<float*>(w + p.head);
+        a.tail = reinterpret_cast<float*>(w + p.tail);
+        a.named = reinterpret_cast<uint8_t*>(w + p.named);
+        return launch_bwd(p, w, a, ids, ids_stride, gtype, dwtype, vec, s);
+    };
+    return ids64 ? run(int64_t{}) : run(int32_t{});
 }

@@ -12,21 +12,24 @@ namespace hgsr {
 
 constexpr float kScaleFloor = 0x1p-100f;
 
+template <typename I>
 struct CacheArgs {
     uint32_t capacity, chunks, width;  // chunks: lanes' pieces of this launch; width: pieces per row
     FastDiv per_row;
-    int64_t row0, D;
+    int64_t row0, n, D;
     int group, glog;                   // group = 1 << glog columns
     uint8_t* codes;
     float* scales;
     int64_t cstride, sstride;
-    RowIds slots;                      // slots.p == nullptr: slot i
+    RowIds<I> slots;                   // slots.p == nullptr: slot i
     void* x;                           // rows written, or the rows that a read fills
     int64_t xstride;
+    int stream;                        // read: the rows are stored past the caches
     const int32_t* last;               // write: the last row of each named slot (nullable)
 };
 
-__device__ __forceinline__ uint32_t slot_of(const CacheArgs& a, int64_t i) {
+template <typename I>
+__device__ __forceinline__ uint32_t slot_of(const CacheArgs<I>& a, int64_t i) {
     if (!a.slots.p) return i < (int64_t)a.capacity ? (uint32_t)i : a.capacity;
     return a.slots.get(i, a.capacity);
 }
@@ -69,14 +72,16 @@ __device__ __forceinline__ void decode4(uint32_t w, float* o) {
 // ------------------------------------------------------------------------------------- write
 
 // the last row that names each slot: cleared where it will be read, then the largest row number
-__global__ __launch_bounds__(256) void slot_clear_kernel(uint32_t n, RowIds slots, uint32_t capacity,
+template <typename I>
+__global__ __launch_bounds__(256) void slot_clear_kernel(uint32_t n, RowIds<I> slots, uint32_t capacity,
                                                          int32_t* __restrict__ last) {
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const uint32_t c = slots.get(i, capacity);
     if (c < capacity) last[c] = -1;
 }
-__global__ __launch_bounds__(256) void slot_last_kernel(uint32_t n, RowIds slots, uint32_t capacity,
+template <typename I>
+__global__ __launch_bounds__(256) void slot_last_kernel(uint32_t n, RowIds<I> slots, uint32_t capacity,
                                                         int32_t* __restrict__ last) {
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
@@ -84,65 +89,86 @@ __global__ __launch_bounds__(256) void slot_last_kernel(uint32_t n, RowIds slots
     if (c < capacity) atomicMax(&last[c], (int32_t)i);
 }
 
-// VEC consecutive columns per lane; ALIGNED: whole pieces, moved as vectors
-template <typename XT, int FMT, int VEC, bool ALIGNED>
-__global__ __launch_bounds__(256) void rowcache_write_kernel(const CacheArgs a) {
-    const uint32_t c = blockIdx.x * 256 + threadIdx.x;
-    const uint32_t r = a.per_row.div(c < a.chunks ? c : 0);
-    const int64_t row = a.row0 + r, col = (int64_t)(c - r * a.per_row.d) * VEC;
-    uint32_t slot = c < a.chunks ? slot_of(a, row) : a.capacity;
-    if (slot < a.capacity && a.last && a.last[slot] != (int32_t)row) slot = a.capacity;
-    const bool on = slot < a.capacity && col < a.D;
-    float x[VEC] = {};
-    if (on) {
-        const XT* p = static_cast<const XT*>(a.x) + row * a.xstride + col;
-        if (ALIGNED) {
-            const Vec<XT, VEC> v = load_vec<XT, VEC>(p);
+// VEC consecutive columns per lane; ALIGNED: whole pieces, moved as vectors.  FEW: no more than
+// kFewSlots rows, whose repeated slots are found here, by a group's lanes among the later rows.
+constexpr int kFewSlots = 1024;
+constexpr int kWritePer = 2;  // pieces per lane, 256 apart
+
+template <typename XT, typename I, int FMT, int VEC, bool ALIGNED, bool FEW>
+__global__ __launch_bounds__(256) void rowcache_write_kernel(const CacheArgs<I> a) {
+    __shared__ uint32_t slots[FEW ? kFewSlots : 1];
+    const uint32_t c0 = xcd_remap(blockIdx.x, gridDim.x) * (256 * kWritePer) + threadIdx.x;
+    const int lanes = a.group / VEC;  // a power of two, <= 32
+    uint32_t slot[kWritePer], r[kWritePer];
+    int64_t col[kWritePer];
+    float x[kWritePer][VEC];
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) x[k] = (float)v.v[k];
+    for (int q = 0; q < kWritePer; ++q) {
+        const uint32_t c = c0 + q * 256;
+        const bool in = c < a.chunks;
+        r[q] = a.per_row.div(in ? c : 0);
+        col[q] = in ? (int64_t)(c - r[q] * a.per_row.d) * VEC : a.D;
+        slot[q] = slot_of(a, a.row0 + r[q]);
+        const XT* p = static_cast<const XT*>(a.x) + (a.row0 + r[q]) * a.xstride + col[q];
+        if (ALIGNED) {
+            Vec<XT, VEC> v{};
+            if (col[q] < a.D) v = load_vec<XT, VEC>(p);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) x[q][k] = (float)v.v[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) x[q][k] = col[q] + k < a.D ? (float)p[k] : 0.0f;
+        }
+    }
+    if (FEW) {
+        const uint32_t n = (uint32_t)a.n;
+        for (uint32_t i = threadIdx.x; i < n; i += 256) slots[i] = slot_of(a, i);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int q = 0; q < kWritePer; ++q) {
+        bool on = col[q] < a.D && slot[q] < a.capacity;
+        if (!FEW && a.last && on) on = a.last[slot[q]] == (int32_t)(a.row0 + r[q]);
+        // the largest magnitude of the group as bits: infinities and NaN lie above every number
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) m = max(m, __float_as_uint(x[q][k]) & 0x7fffffffu);
+        if (FEW)  // a later row of the same slot: a mark above every magnitude
+            for (uint32_t j = (uint32_t)a.row0 + r[q] + 1 + (threadIdx.x & (lanes - 1)); j < (uint32_t)a.n; j += lanes)
+                if (slots[j] == slot[q]) m = 0x80000000u;
+        for (int d = 1; d < lanes; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+        if (!on || (FEW && m == 0x80000000u)) continue;
+        const bool finite = m < 0x7f800000u;
+        const float per = FMT == HGSR_INT8 ? 1.0f / 127.0f : 1.0f / 448.0f;
+        const float s = fmaxf(__uint_as_float(m) * per, kScaleFloor), inv = 1.0f / s;
+        uint32_t w[VEC / 4];
+#pragma unroll
+        for (int k = 0; k < VEC; k += 4) {
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = finite ? quotient_odd(x[q][k + j], s, inv) : 0.0f;
+            w[k / 4] = encode4<FMT>(y[0], y[1], y[2], y[3]);
+        }
+        uint8_t* to = a.codes + (int64_t)slot[q] * a.cstride + col[q];
+        if (ALIGNED) {
+            Vec<uint32_t, VEC / 4> o;
+#pragma unroll
+            for (int k = 0; k < VEC / 4; ++k) o.v[k] = w[k];
+            store_vec<uint32_t, VEC / 4>(reinterpret_cast<uint32_t*>(to), o);
         } else {
 #pragma unroll
             for (int k = 0; k < VEC; ++k)
-                if (col + k < a.D) x[k] = (float)p[k];
+                if (col[q] + k < a.D) to[k] = (uint8_t)(w[k / 4] >> (8 * (k & 3)));
         }
+        if ((col[q] & (a.group - 1)) == 0)
+            a.scales[(int64_t)slot[q] * a.sstride + (col[q] >> a.glog)] = finite ? s : __builtin_nanf("");
     }
-    // the largest magnitude of the group as bits: infinities and NaN lie above every number
-    uint32_t m = 0;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) m = max(m, __float_as_uint(x[k]) & 0x7fffffffu);
-    const int lanes = a.group / VEC;  // a power of two, <= 32
-    for (int d = 1; d < lanes; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
-    if (!on) return;
-    const bool finite = m < 0x7f800000u;
-    const float per = FMT == HGSR_INT8 ? 1.0f / 127.0f : 1.0f / 448.0f;
-    const float s = fmaxf(__uint_as_float(m) * per, kScaleFloor), inv = 1.0f / s;
-    uint32_t w[VEC / 4];
-#pragma unroll
-    for (int k = 0; k < VEC; k += 4) {
-        float q[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = finite ? quotient_odd(x[k + j], s, inv) : 0.0f;
-        w[k / 4] = encode4<FMT>(q[0], q[1], q[2], q[3]);
-    }
-    uint8_t* to = a.codes + (int64_t)slot * a.cstride + col;
-    if (ALIGNED) {
-        Vec<uint32_t, VEC / 4> o;
-#pragma unroll
-        for (int k = 0; k < VEC / 4; ++k) o.v[k] = w[k];
-        store_vec<uint32_t, VEC / 4>(reinterpret_cast<uint32_t*>(to), o);
-    } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k)
-            if (col + k < a.D) to[k] = (uint8_t)(w[k / 4] >> (8 * (k & 3)));
-    }
-    if ((col & (a.group - 1)) == 0)
-        a.scales[(int64_t)slot * a.sstride + (col >> a.glog)] = finite ? s : __builtin_nanf("");
 }
 
 // -------------------------------------------------------------------------------------- read
 
-template <typename OT, int FMT, int VEC, bool ALIGNED>
-__global__ __launch_bounds__(256) void rowcache_read_kernel(const CacheArgs a) {
+template <typename OT, typename I, int FMT, int VEC, bool ALIGNED>
+__global__ __launch_bounds__(256) void rowcache_read_kernel(const CacheArgs<I> a) {
     const uint32_t c = blockIdx.x * 256 + threadIdx.x;
     if (c >= a.chunks) return;
     const uint32_t r = a.per_row.div(c);
@@ -174,7 +200,10 @@ __global__ __launch_bounds__(256) void rowcache_read_kernel(const CacheArgs a) {
         Vec<OT, VEC> o;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o.v[k] = (OT)x[k];
-        store_vec<OT, VEC>(to, o);
+        if (a.stream)
+            stream_vec<OT, VEC>(to, o);
+        else
+            store_vec<OT, VEC>(to, o);
     } else {
 #pragma unroll
         for (int k = 0; k < VEC; ++k)
@@ -184,29 +213,32 @@ __global__ __launch_bounds__(256) void rowcache_read_kernel(const CacheArgs a) {
 
 // ---------------------------------------------------------------------------------- launches
 
-template <typename T, int FMT, int VEC>
-static void launch(bool write, bool aligned, const CacheArgs& a, hipStream_t s) {
-    const dim3 grid((a.chunks + 255) / 256), block(256);
-    if (write && aligned)
-        hipLaunchKernelGGL((rowcache_write_kernel<T, FMT, VEC, true>), grid, block, 0, s, a);
-    else if (write)
-        hipLaunchKernelGGL((rowcache_write_kernel<T, FMT, VEC, false>), grid, block, 0, s, a);
-    else if (aligned)
-        hipLaunchKernelGGL((rowcache_read_kernel<T, FMT, VEC, true>), grid, block, 0, s, a);
+template <typename T, int FMT, int VEC, bool ALIGNED, typename I>
+static void launch(bool write, const CacheArgs<I>& a, hipStream_t s) {
+    const dim3 block(256), wgrid((a.chunks + 256 * kWritePer - 1) / (256 * kWritePer)), rgrid((a.chunks + 255) / 256);
+    if (!write)
+        hipLaunchKernelGGL((rowcache_read_kernel<T, I, FMT, VEC, ALIGNED>), rgrid, block, 0, s, a);
+    else if (a.slots.p && a.n > 1 && a.n <= kFewSlots)
+        hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, ALIGNED, true>), wgrid, block, 0, s, a);
     else
-        hipLaunchKernelGGL((rowcache_read_kernel<T, FMT, VEC, false>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, ALIGNED, false>), wgrid, block, 0, s, a);
 }
 
-template <typename T, int VEC>
-static void launch(bool write, int format, int64_t n, CacheArgs a, hipStream_t s) {
+template <typename T, int FMT, int VEC, typename I>
+static void launch(bool write, bool aligned, const CacheArgs<I>& a, hipStream_t s) {
+    return aligned ? launch<T, FMT, VEC, true>(write, a, s) : launch<T, FMT, VEC, false>(write, a, s);
+}
+
+template <typename T, int VEC, typename I>
+static void launch(bool write, int format, CacheArgs<I> a, hipStream_t s) {
     bool aligned = a.D % VEC == 0 && a.cstride % VEC == 0 && (uintptr_t)a.codes % VEC == 0;
     aligned = aligned && (uintptr_t)a.x % 16 == 0 && a.xstride % VEC == 0;
     // a write's rows are whole groups of lanes, so that no group crosses a wave
     const int64_t per_row = write ? (a.D + a.group - 1) / a.group * (a.group / VEC) : (a.D + VEC - 1) / VEC;
     const int64_t most = ((int64_t)1 << 30) / per_row;
     a.per_row = fast_div((uint32_t)per_row);
-    for (a.row0 = 0; a.row0 < n; a.row0 += most) {
-        a.chunks = (uint32_t)((n - a.row0 < most ? n - a.row0 : most) * per_row);
+    for (a.row0 = 0; a.row0 < a.n; a.row0 += most) {
+        a.chunks = (uint32_t)((a.n - a.row0 < most ? a.n - a.row0 : most) * per_row);
         if (format == HGSR_INT8)
             launch<T, HGSR_INT8, VEC>(write, aligned, a, s);
         else
@@ -214,94 +246,108 @@ static void launch(bool write, int format, int64_t n, CacheArgs a, hipStream_t s
     }
 }
 
-static void launch(bool write, int type, int format, int64_t n, const CacheArgs& a, hipStream_t s) {
-    if (type == HGSR_F32)
-        launch<float, 4>(write, format, n, a, s);
-    else if (type == HGSR_F16)
-        launch<f16_t, 8>(write, format, n, a, s);
+// the call's arguments that no kernel template hangs on
+struct CacheCall {
+    int64_t capacity, n, D, cstride, sstride, slots_stride, xstride;
+    int group, format, type, slots64;
+    const void* slots;
+    void *codes, *x, *ws;
+    float* scales;
+};
+
+template <typename I>
+static void launch(bool write, const CacheCall& c, hipStream_t s) {
+    CacheArgs<I> a{};
+    a.capacity = (uint32_t)c.capacity;
+    a.n = c.n;
+    a.D = c.D;
+    a.group = c.group;
+    a.glog = c.group == 16 ? 4 : c.group == 32 ? 5 : c.group == 64 ? 6 : 7;
+    a.codes = static_cast<uint8_t*>(c.codes);
+    a.scales = c.scales;
+    a.cstride = c.cstride;
+    a.sstride = c.sstride;
+    a.slots = RowIds<I>{static_cast<const I*>(c.slots), c.slots_stride};
+    a.x = c.x;
+    a.xstride = c.xstride;
+    a.stream = stream_out(c.n * c.D * elem_size(c.type));
+    if (write && c.slots && c.n > kFewSlots) {
+        int32_t* last = static_cast<int32_t*>(c.ws);
+        const dim3 grid((unsigned)((c.n + 255) / 256));
+        hipLaunchKernelGGL((slot_clear_kernel<I>), grid, dim3(256), 0, s, (uint32_t)c.n, a.slots, a.capacity, last);
+        hipLaunchKernelGGL((slot_last_kernel<I>), grid, dim3(256), 0, s, (uint32_t)c.n, a.slots, a.capacity, last);
+        a.last = last;
+    }
+    if (c.type == HGSR_F32)
+        launch<float, 4>(write, c.format, a, s);
+    else if (c.type == HGSR_F16)
+        launch<f16_t, 8>(write, c.format, a, s);
     else
-        launch<bf16_t, 8>(write, format, n, a, s);
+        launch<bf16_t, 8>(write, c.format, a, s);
+}
+
+static void launch(bool write, const CacheCall& c, hipStream_t s) {
+    return c.slots64 ? launch<int64_t>(write, c, s) : launch<int32_t>(write, c, s);
 }
 
 }  // namespace hgsr
 
 using namespace hgsr;
 
-static int cache_args(const char* what, int64_t capacity, int64_t n, int64_t D, int group, int format, int type,
-                      int64_t cstride, int64_t sstride, const void* slots, int slots64, int64_t slots_stride,
-                      CacheArgs& a) {
-    HGSR_REQUIRE(capacity >= 0 && capacity < (1ll << 31), "%s: capacity %lld outside [0, 2^31)", what,
-                 (long long)capacity);
-    HGSR_REQUIRE(n >= 0 && n < (1ll << 31) - 256, "%s: %lld rows: too many", what, (long long)n);
-    HGSR_REQUIRE(D >= 1 && D <= (1ll << 21), "%s: row length %lld outside [1, 2^21]", what, (long long)D);
-    HGSR_REQUIRE(group == 16 || group == 32 || group == 64 || group == 128, "%s: group of %d columns (16, 32, 64, 128)",
-                 what, group);
-    HGSR_REQUIRE(format == HGSR_INT8 || format == HGSR_E4M3, "%s: unknown format", what);
-    HGSR_REQUIRE(type_ok(type), "%s: unknown element type", what);
-    HGSR_REQUIRE(cstride >= D && sstride >= (D + group - 1) / group && slots_stride >= 0, "%s: bad stride", what);
-    HGSR_REQUIRE(slots || n <= capacity, "%s: %lld rows, %lld slots", what, (long long)n, (long long)capacity);
-    a.capacity = (uint32_t)capacity;
-    a.D = D;
-    a.group = group;
-    a.glog = group == 16 ? 4 : group == 32 ? 5 : group == 64 ? 6 : 7;
-    a.cstride = cstride;
-    a.sstride = sstride;
-    a.slots = RowIds{slots, slots_stride, slots64};
+static int check_cache(const char* what, const CacheCall& c) {
+    HGSR_REQUIRE(c.capacity >= 0 && c.capacity < (1ll << 31), "%s: capacity %lld outside [0, 2^31)", what,
+                 (long long)c.capacity);
+    HGSR_REQUIRE(c.n >= 0 && c.n < (1ll << 31) - 4096, "%s: %lld rows: too many", what, (long long)c.n);
+    HGSR_REQUIRE(c.D >= 1 && c.D <= (1ll << 21), "%s: row length %lld outside [1, 2^21]", what, (long long)c.D);
+    HGSR_REQUIRE(c.group == 16 || c.group == 32 || c.group == 64 || c.group == 128,
+                 "%s: group of %d columns (16, 32, 64, 128)", what, c.group);
+    HGSR_REQUIRE(c.format == HGSR_INT8 || c.format == HGSR_E4M3, "%s: unknown format", what);
+    HGSR_REQUIRE(type_ok(c.type), "%s: unknown element type", what);
+    HGSR_REQUIRE(c.cstride >= c.D && c.sstride >= (c.D + c.group - 1) / c.group && c.slots_stride >= 0 && c.xstride >= 0,
+                 "%s: bad stride", what);
+    HGSR_REQUIRE(c.slots || c.n <= c.capacity, "%s: %lld rows, %lld slots", what, (long long)c.n,
+                 (long long)c.capacity);
     return HGSR_OK;
 }
 
 extern "C" size_t hgsr_rowcache_write_ws_bytes(int64_t capacity, int64_t n, int has_slots) {
-    return has_slots && n > 1 && capacity > 0 ? (size_t)capacity * sizeof(int32_t) : 0;
+    return has_slots && n > kFewSlots && capacity > 0 ? (size_t)capacity * sizeof(int32_t) : 0;
 }
 
 extern "C" int hgsr_rowcache_write(int64_t capacity, int64_t n, int64_t D, int group, int format, const void* x,
                                    int xtype, int64_t xstride, const void* slots, int slots64, int64_t slots_stride,
                                    void* codes, int64_t cstride, float* scales, int64_t sstride, void* ws,
                                    size_t ws_bytes, hgsr_stream_t stream) {
-    CacheArgs a{};
-    if (int st = cache_args("rowcache_write", capacity, n, D, group, format, xtype, cstride, sstride, slots, slots64,
-                            slots_stride, a))
-        return st;
-    HGSR_REQUIRE(xstride >= 0, "rowcache_write: negative stride");
+    const CacheCall c{capacity, n,      D,     cstride, sstride, slots_stride, xstride,
+                      group,    format, xtype, slots64, slots,   codes,        const_cast<void*>(x), ws, scales};
+    if (int st = check_cache("rowcache_write", c)) return st;
     if (n == 0 || capacity == 0) return HGSR_OK;
     HGSR_REQUIRE(x && codes && scales, "rowcache_write: null pointer");
-    a.x = const_cast<void*>(x);
-    a.xstride = xstride;
-    a.codes = static_cast<uint8_t*>(codes);
-    a.scales = scales;
-    hipStream_t s = as_stream(stream);
-    KernelTimer kt("rowcache_write", s);
-    if (slots && n > 1) {
-        const size_t need = hgsr_rowcache_write_ws_bytes(capacity, n, 1);
-        if (!ws || ws_bytes < need) {
-            set_error("rowcache_write: workspace of %zu bytes, %zu needed", ws_bytes, need);
-            return HGSR_EWORKSPACE;
-        }
-        int32_t* last = static_cast<int32_t*>(ws);
-        const dim3 grid((unsigned)((n + 255) / 256));
-        hipLaunchKernelGGL(slot_clear_kernel, grid, dim3(256), 0, s, (uint32_t)n, a.slots, a.capacity, last);
-        hipLaunchKernelGGL(slot_last_kernel, grid, dim3(256), 0, s, (uint32_t)n, a.slots, a.capacity, last);
-        a.last = last;
+    const size_t need = hgsr_rowcache_write_ws_bytes(capacity, n, slots != nullptr);
+    if (need > ws_bytes || (need && !ws)) {
+        set_error("rowcache_write: workspace of %zu bytes, %zu needed", ws ? ws_bytes : (size_t)0, need);
+        return HGSR_EWORKSPACE;
     }
-    launch(true, xtype, format, n, a, s);
+    hipStream_t s = as_stream(stream);
+    {
+        KernelTimer kt("rowcache_write", s);
+        launch(true, c, s);
+    }
     return check_launch("rowcache_write");
 }
 
 extern "C" int hgsr_rowcache_read(int64_t capacity, int64_t n, int64_t D, int group, int format, const void* codes,
                                   int64_t cstride, const float* scales, int64_t sstride, const void* slots,
                                   int slots64, int64_t slots_stride, void* out, int otype, hgsr_stream_t stream) {
-    CacheArgs a{};
-    if (int st = cache_args("rowcache_read", capacity, n, D, group, format, otype, cstride, sstride, slots, slots64,
-                            slots_stride, a))
-        return st;
+    const CacheCall c{capacity, n,      D,     cstride, sstride, slots_stride, D, group, format, otype, slots64, slots,
+                      const_cast<void*>(codes), out, nullptr, const_cast<float*>(scales)};
+    if (int st = check_cache("rowcache_read", c)) return st;
     if (n == 0) return HGSR_OK;
     HGSR_REQUIRE(out && (capacity == 0 || (codes && scales)), "rowcache_read: null pointer");
-    a.x = out;
-    a.xstride = D;
-    a.codes = const_cast<uint8_t*>(static_cast<const uint8_t*>(codes));
-    a.scales = const_cast<float*>(scales);
     hipStream_t s = as_stream(stream);
-    KernelTimer kt("rowcache_read", s);
-    launch(false, otype, format, n, a, s);
+    {
+        KernelTimer kt("rowcache_read", s);
+        launch(false, c, s);
+    }
     return check_launch("rowcache_read");
 }

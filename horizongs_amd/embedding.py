@@ -13,7 +13,6 @@ so they are the same bits on every run.  There is no CPU path.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from . import gradbuf
@@ -21,13 +20,18 @@ from . import gradbuf
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
+_IDS = {torch.int32: 0, torch.int64: 1}
+
+
 def check_device(*ts):
-    dev = ts[0].device
+    """The device number of tensors that all lie on one HIP device."""
+    index = ts[0].get_device()
     for t in ts:
         if not t.is_cuda:
             raise RuntimeError("hgsr: inputs must be HIP device tensors (no CPU fallback)")
-        if t.device != dev:
-            raise RuntimeError(f"hgsr: tensors on {dev} and {t.device}: one device is needed")
+        if t.get_device() != index:
+            raise RuntimeError(f"hgsr: tensors on devices {index} and {t.get_device()}: one is needed")
+    return index
 
 
 def type_code(dtype):
@@ -39,72 +43,96 @@ def type_code(dtype):
 
 def row_stride(t, what):
     """Elements between the rows of a 2-D tensor whose columns are contiguous."""
-    if t.shape[1] > 1 and t.stride(1) != 1 and t.numel():
-        raise ValueError(f"hgsr: the columns of {what} must be contiguous (stride {t.stride(1)})")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    n, d = t.shape
+    s0, s1 = t.stride()
+    if s1 != 1 and d > 1 and n:
+        raise ValueError(f"hgsr: the columns of {what} must be contiguous (stride {s1})")
+    return s0 if n > 1 else d
 
 
 def rows_view(t, dim, what):
     """[n, dim] view of a tensor's rows with contiguous columns, copied only if there is none."""
     if t.shape[-1] != dim:
         raise ValueError(f"hgsr: rows of {what} have {t.shape[-1]} columns, not {dim}")
-    t = t.reshape(-1, dim)
+    if t.dim() != 2:
+        t = t.reshape(-1, dim)
     return t if dim == 1 or t.stride(1) == 1 else t.contiguous()
 
 
 def check_ids(ids):
-    if ids.dtype not in (torch.int32, torch.int64):
+    """1 for int64 ids, 0 for int32."""
+    is64 = _IDS.get(ids.dtype)
+    if is64 is None:
         raise ValueError(f"hgsr: int32 or int64 ids are needed, not {ids.dtype}")
+    return is64
 
 
-def id_args(ids):
-    """(flat ids, whether they are int64, their stride)."""
-    flat = ids.reshape(-1)
-    return flat, int(ids.dtype == torch.int64), flat.stride(0) if flat.numel() > 1 else 1
+def flat_ids(ids):
+    return ids if ids.dim() == 1 else ids.reshape(-1)
 
 
-def _lookup(weight, ids, scale, dtype):
+def id_stride(flat):
+    return flat.stride(0) if flat.shape[0] > 1 else 1
+
+
+def _lookup(weight, flat, shape, scale, dtype, index):
     V, D = weight.shape
-    out = torch.empty(*ids.shape, D, dtype=dtype, device=weight.device)
-    n = ids.numel()
+    out = weight.new_empty((*shape, D), dtype=dtype)
+    n = flat.shape[0]
     if n and D:
-        flat, is64, stride = id_args(ids)
-        N.call_on(weight.device, "hgsr_embed_fwd", V, n, D, weight.data_ptr(), _TYPES[weight.dtype],
-                  row_stride(weight, "weight"), flat.data_ptr(), is64, stride, scale, out.data_ptr(), _TYPES[dtype])
+        N.call_on(index, "hgsr_embed_fwd", V, n, D, weight.data_ptr(), _TYPES[weight.dtype],
+                  row_stride(weight, "weight"), flat.data_ptr(), _IDS[flat.dtype], id_stride(flat), scale,
+                  out.data_ptr(), _TYPES[dtype])
     return out
 
 
-def _grad(grad, ids, out, scale, accumulate):
+def _grad(grad, flat, out, scale, accumulate, index):
     V, D = out.shape
-    n = ids.numel()
+    n = flat.shape[0]
     if V == 0 or D == 0 or (n == 0 and accumulate):
         return out
-    flat, is64, stride = id_args(ids)
     ws_b = N.size_query("hgsr_embed_bwd_ws_bytes", V, n, D)
-    ws = torch.empty(max(ws_b, 1), dtype=torch.uint8, device=out.device)
-    N.call_on(out.device, "hgsr_embed_bwd", V, n, D, grad.data_ptr(), _TYPES[grad.dtype], row_stride(grad, "grad"),
-              flat.data_ptr(), is64, stride, scale, out.data_ptr(), _TYPES[out.dtype], row_stride(out, "out"),
-              int(accumulate), ws.data_ptr(), ws_b)
+    ws = torch.empty(ws_b, dtype=torch.uint8, device=out.device) if ws_b else None
+    N.call_on(index, "hgsr_embed_bwd", V, n, D, grad.data_ptr(), _TYPES[grad.dtype], row_stride(grad, "grad"),
+              flat.data_ptr(), _IDS[flat.dtype], id_stride(flat), scale, out.data_ptr(), _TYPES[out.dtype],
+              row_stride(out, "out"), int(accumulate), ws.data_ptr() if ws_b else None, ws_b)
     return out
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, ids, scale, dtype):
-        ctx.save_for_backward(ids)
-        ctx.table = (weight.shape, weight.dtype, gradbuf.key(weight))
-        ctx.scale = scale
-        return _lookup(weight, ids, scale, dtype)
+    def forward(ctx, weight, flat, shape, scale, dtype, index):
+        ctx.save_for_backward(flat)
+        ctx.args = (weight.shape, weight.dtype, gradbuf.key(weight), scale, index)
+        return _lookup(weight, flat, shape, scale, dtype, index)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        (ids,) = ctx.saved_tensors
-        shape, dtype, key = ctx.table
+        (flat,) = ctx.saved_tensors
+        shape, dtype, key, scale, index = ctx.args
+        if torch.is_grad_enabled():  # create_graph: the gradient is linear in g, and its own gradient a lookup
+            return _EmbeddingGrad.apply(g, flat, shape, dtype, scale, index), None, None, None, None, None
         out = gradbuf.take(key, shape, dtype)  # in place in a DDP bucket when one is registered
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=g.device)
-        return _grad(rows_view(g, shape[1], "grad"), ids, out, ctx.scale, False), None, None, None
+            out = g.new_empty(shape, dtype=dtype)
+        return _grad(rows_view(g, shape[1], "grad"), flat, out, scale, False, index), None, None, None, None, None
+
+
+class _EmbeddingGrad(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, g, flat, shape, dtype, scale, index):
+        ctx.save_for_backward(flat)
+        ctx.args = (g.shape, g.dtype, scale, index)
+        return _grad(rows_view(g, shape[1], "grad"), flat, g.new_empty(shape, dtype=dtype), scale, False, index)
+
+    @staticmethod
+    def backward(ctx, gg):
+        (flat,) = ctx.saved_tensors
+        shape, dtype, scale, index = ctx.args
+        gg = rows_view(gg, gg.shape[1], "the gradient's gradient")
+        if torch.is_grad_enabled():
+            return _Embedding.apply(gg, flat, shape[:-1], scale, dtype, index), None, None, None, None, None
+        return _lookup(gg, flat, shape[:-1], scale, dtype, index), None, None, None, None, None
 
 
 def embedding(weight, ids, scale=1.0, dtype=None):
@@ -113,14 +141,18 @@ def embedding(weight, ids, scale=1.0, dtype=None):
     once.  Differentiable in weight; the gradient has weight's type and a row for each of its rows."""
     if weight.dim() != 2:
         raise ValueError(f"hgsr: weight must be [rows, columns], not {tuple(weight.shape)}")
-    dtype = weight.dtype if dtype is None else dtype
-    type_code(weight.dtype), type_code(dtype)
+    type_code(weight.dtype)
+    if dtype is None:
+        dtype = weight.dtype
+    else:
+        type_code(dtype)
     row_stride(weight, "weight")
     check_ids(ids)
-    check_device(weight, ids)
+    index = check_device(weight, ids)
+    flat = flat_ids(ids)
     if weight.requires_grad and torch.is_grad_enabled():
-        return _Embedding.apply(weight, ids, float(scale), dtype)
-    return _lookup(weight, ids, float(scale), dtype)
+        return _Embedding.apply(weight, flat, ids.shape, float(scale), dtype, index)
+    return _lookup(weight, flat, ids.shape, float(scale), dtype, index)
 
 
 @torch.no_grad()
@@ -141,17 +173,18 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
     if out is None:
         dtype = grad.dtype if dtype is None else dtype
         type_code(dtype)
-        check_device(grad, ids)
-        g = rows_view(grad, D, "grad") if D else grad
-        return _grad(g, ids, torch.empty(num_rows, D, dtype=dtype, device=grad.device), float(scale), False)
-    type_code(out.dtype)
-    if tuple(out.shape) != (num_rows, D) or (dtype is not None and dtype != out.dtype):
-        raise ValueError(f"hgsr: out is {tuple(out.shape)} of {out.dtype}, not {(num_rows, D)} of {dtype or 'its type'}")
-    if row_stride(out, "out") < D:
-        raise ValueError("hgsr: the rows of out overlap")
-    check_device(grad, ids, out)
+        index = check_device(grad, ids)
+        out, accumulate = grad.new_empty((num_rows, D), dtype=dtype), False
+    else:
+        type_code(out.dtype)
+        if tuple(out.shape) != (num_rows, D) or (dtype is not None and dtype != out.dtype):
+            raise ValueError(f"hgsr: out is {tuple(out.shape)} of {out.dtype}, not {(num_rows, D)} of "
+                             f"{dtype or 'its type'}")
+        if row_stride(out, "out") < D:
+            raise ValueError("hgsr: the rows of out overlap")
+        index, accumulate = check_device(grad, ids, out), True
     g = rows_view(grad, D, "grad") if D else grad
-    return _grad(g, ids, out, float(scale), True)
+    return _grad(g, flat_ids(ids), out, float(scale), accumulate, index)
 
 
 class Embedding(torch.nn.Module):

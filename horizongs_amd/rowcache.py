@@ -20,7 +20,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native as N
-from .embedding import _TYPES, check_device, check_ids, id_args, row_stride, rows_view, type_code
+from .embedding import _TYPES, check_device, check_ids, id_stride, row_stride, type_code
 
 _FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _NAMES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
@@ -61,14 +61,16 @@ def _cache(cache):
     return codes, scales, group, cs, ss
 
 
-def _slots(slots, n):
+def _slot_args(slots):
     if slots is None:
-        return None, None, 0, 1
+        return None, 0, 1
+    return slots.data_ptr(), int(slots.dtype == torch.int64), id_stride(slots)
+
+
+def _check_slots(slots, n):
     if slots.dim() != 1 or (n is not None and slots.shape[0] != n):
         raise ValueError(f"hgsr row cache: slots {tuple(slots.shape)}: [n] is needed, one number for each row")
     check_ids(slots)
-    flat, is64, stride = id_args(slots)
-    return flat, flat.data_ptr(), is64, stride
 
 
 @torch.no_grad()
@@ -78,24 +80,25 @@ def rowcache_write(cache, rows, slots=None):
     out; where a slot is named twice, the last of its rows stays.  Other slots keep what they hold.  A
     write is ordered on the current stream like any kernel; two streams must not write one slot at once."""
     codes, scales, group, cs, ss = _cache(cache)
-    type_code(rows.dtype)
+    xt = type_code(rows.dtype)
     capacity, dim = codes.shape
     if rows.dim() != 2 or rows.shape[1] != dim:
         raise ValueError(f"hgsr row cache: rows {tuple(rows.shape)}: [n, {dim}] are needed")
     n = rows.shape[0]
-    if slots is None and n > capacity:
-        raise ValueError(f"hgsr row cache: {n} rows, {capacity} slots")
-    keep, sp, is64, stride = _slots(slots, n)
-    check_device(codes, scales, rows, *(() if slots is None else (slots,)))
+    xs = row_stride(rows, "rows")
+    if slots is None:
+        if n > capacity:
+            raise ValueError(f"hgsr row cache: {n} rows, {capacity} slots")
+        index = check_device(codes, scales, rows)
+    else:
+        _check_slots(slots, n)
+        index = check_device(codes, scales, rows, slots)
     if n == 0 or capacity == 0:
         return
-    x = rows_view(rows, dim, "rows")
     ws_b = N.size_query("hgsr_rowcache_write_ws_bytes", capacity, n, int(slots is not None))
     ws = torch.empty(ws_b, dtype=torch.uint8, device=codes.device) if ws_b else None
-    N.call_on(codes.device, "hgsr_rowcache_write", capacity, n, dim, group, _FORMATS[codes.dtype], x.data_ptr(),
-              _TYPES[x.dtype], row_stride(x, "rows"), sp, is64, stride, codes.data_ptr(), cs, scales.data_ptr(), ss,
-              None if ws is None else ws.data_ptr(), ws_b)
-    del keep
+    N.call_on(index, "hgsr_rowcache_write", capacity, n, dim, group, _FORMATS[codes.dtype], rows.data_ptr(), xt, xs,
+              *_slot_args(slots), codes.data_ptr(), cs, scales.data_ptr(), ss, ws.data_ptr() if ws_b else None, ws_b)
 
 
 @torch.no_grad()
@@ -103,14 +106,15 @@ def rowcache_read(cache, slots=None, dtype=torch.float32):
     """Rows [n, dim] of the named slots (int32 / int64 [n]; None: every slot) in `dtype`: code * scale in
     f32, rounded once.  A slot outside the cache reads zeros."""
     codes, scales, group, cs, ss = _cache(cache)
-    type_code(dtype)
+    ot = type_code(dtype)
     capacity, dim = codes.shape
-    keep, sp, is64, stride = _slots(slots, None)
-    check_device(codes, scales, *(() if slots is None else (slots,)))
-    n = capacity if slots is None else slots.shape[0]
-    out = torch.empty(n, dim, dtype=dtype, device=codes.device)
+    if slots is None:
+        n, index = capacity, check_device(codes, scales)
+    else:
+        _check_slots(slots, None)
+        n, index = slots.shape[0], check_device(codes, scales, slots)
+    out = scales.new_empty((n, dim), dtype=dtype)
     if n:
-        N.call_on(codes.device, "hgsr_rowcache_read", capacity, n, dim, group, _FORMATS[codes.dtype], codes.data_ptr(),
-                  cs, scales.data_ptr(), ss, sp, is64, stride, out.data_ptr(), _TYPES[dtype])
-    del keep
+        N.call_on(index, "hgsr_rowcache_read", capacity, n, dim, group, _FORMATS[codes.dtype], codes.data_ptr(), cs,
+                  scales.data_ptr(), ss, *_slot_args(slots), out.data_ptr(), ot)
     return out

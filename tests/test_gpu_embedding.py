@@ -222,9 +222,13 @@ def test_autograd_and_differences():
     o = E.embedding(b, ids, 1.0, dtype=F32)
     o.backward(torch.ones_like(o))
     assert o.dtype == F32 and b.grad.dtype == BF16
-    with pytest.raises(RuntimeError):  # a second derivative is not offered
-        (x,) = torch.autograd.grad(E.embedding(w, ids).square().sum(), w, create_graph=True)
-        x.sum().backward()
+    # second derivatives: of sum((s W[ids])^2 c) / 2 along d, 2 s^2 sum c d[ids] back to its rows
+    q = w.detach().clone().requires_grad_(True)
+    (x,) = torch.autograd.grad((E.embedding(q, ids, scale).square() * c).sum(), q, create_graph=True)
+    (hd,) = torch.autograd.grad(x, q, d)
+    gd = (2 * c.double() * want_lookup(d.cpu(), ids.cpu(), scale).to(DEV)).cpu().reshape(n, D)
+    s, m, run = want_grad(gd, ids.cpu().reshape(-1), V, scale)
+    check(hd, s, (run + 4) * U * m)
 
 
 def test_gradient_lands_in_a_registered_destination():
