@@ -17,10 +17,10 @@ namespace hgsr {
 
 // ------------------------------------------------------------------------------------- lookup
 
-template <typename WT, typename OT, typename I, int VEC>
+template <typename WT, typename OT, typename I, int VEC, bool STREAM>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(uint32_t chunks, FastDiv per_row, uint32_t V,
                                                         const WT* __restrict__ w, int64_t wstride, RowIds<I> ids,
-                                                        int64_t row0, float scale, OT* __restrict__ out, int stream) {
+                                                        int64_t row0, float scale, OT* __restrict__ out) {
     const uint32_t c = blockIdx.x * 256 + threadIdx.x;
     if (c >= chunks) return;
     const uint32_t r = per_row.div(c), col = (c - r * per_row.d) * VEC;
@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(uint32_t chunks, FastDiv
         for (int k = 0; k < VEC; ++k) o.v[k] = (OT)0.0f;
     }
     OT* to = out + (row0 + r) * ((int64_t)per_row.d * VEC) + col;
-    if (stream)
+    if (STREAM)
         stream_vec<OT, VEC>(to, o);
     else
         store_vec<OT, VEC>(to, o);
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(uint32_t chunks, FastDiv
 struct ZeroPart {
     uint4* p;        // whole 16-byte units
     int64_t units;
-    uint16_t* edge[2];  // what lies before the first and behind the last unit (part 0 only)
+    uint16_t* edge[2];  // what lies before the first and behind the last unit
     int nedge[2];
 };
 constexpr int kZeroUnits = 2048;  // per workgroup and turn: 32 KB
@@ -107,14 +107,15 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {  // inclus
 constexpr int kBucketMost = 16384;
 constexpr int kBucketRounds = kBucketMost / 1024;
 constexpr int kBucketLog = 8;
-constexpr int kBucketBits = 8;  // per pass
+constexpr int kBucketBits = 9;  // per pass
+constexpr int kCountMost = 512;  // entries that a workgroup sorts by counting
 
 template <typename I>
 __global__ __launch_bounds__(1024) void sort_bucket_kernel(uint32_t n, RowIds<I> ids, uint32_t V, int shift, int passes,
                                                            int bits, uint2* __restrict__ out, uint32_t buckets,
                                                            ZeroPart zeros) {
     __shared__ uint16_t pos[kBucketMost];
-    __shared__ uint32_t cnt[16][1 << kBucketBits];
+    __shared__ __align__(16) uint32_t cnt[16][1 << kBucketBits];
     __shared__ uint32_t wsum[2][16];
     if (blockIdx.x >= buckets) return store_zeros<1024>(zeros, blockIdx.x - buckets, gridDim.x - buckets);
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
@@ -160,6 +161,30 @@ __global__ __launch_bounds__(1024) void sort_bucket_kernel(uint32_t n, RowIds<I>
     if (passes == 0) {  // a range of one id
         for (int r = 0; r < rounds; ++r)
             if (base + r * 64 < m) out[base + r * 64] = make_uint2(blockIdx.x, pos[base + r * 64]);
+        return;
+    }
+    if (m <= kCountMost) {
+        // few: an entry's place is the number of entries before it, each comparing with all; `parts`
+        // threads share an entry's comparisons
+        uint32_t *id = cnt[0], *before = cnt[0] + kCountMost;
+        const uint32_t width = m <= 64 ? 64 : m <= 128 ? 128 : m <= 256 ? 256 : 512, parts = 1024 / width;
+        if ((uint32_t)tid < width) {
+            id[tid] = (uint32_t)tid < m ? ids.get(pos[tid], V) : ~0u;
+            before[tid] = 0;
+        }
+        __syncthreads();
+        const uint32_t i = tid & (width - 1), own = id[i], share = width / parts, j0 = (tid / width) * share;
+        uint32_t sum = 0;
+        for (uint32_t j = j0; j < j0 + share; j += 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(id + j);
+            sum += v.x < own + (j < i);
+            sum += v.y < own + (j + 1 < i);
+            sum += v.z < own + (j + 2 < i);
+            sum += v.w < own + (j + 3 < i);
+        }
+        if (i < m) atomicAdd(&before[i], sum);
+        __syncthreads();
+        if ((uint32_t)tid < m) out[before[tid]] = make_uint2(own, pos[tid]);
         return;
     }
     const uint32_t bins = 1u << bits;
@@ -250,28 +275,30 @@ __device__ __forceinline__ uint2 sort_entry(const SortArgs<I>& a, uint32_t i) {
 template <bool FIRST, typename I>
 __global__ __launch_bounds__(256) void sort_count_kernel(const SortArgs<I> a, ZeroPart zeros) {
     __shared__ uint32_t h[1 << kSortBits];
-    if (blockIdx.x >= a.tiles) return store_zeros<256>(zeros, blockIdx.x - a.tiles, gridDim.x - a.tiles);
+    __shared__ uint32_t id[FIRST ? kSortTile + 1 : 1];
     if (!FIRST && *a.ascend) return;
+    if (blockIdx.x >= a.tiles) return store_zeros<256>(zeros, blockIdx.x - a.tiles, gridDim.x - a.tiles);
     const uint32_t bins = 1u << a.bits, base = blockIdx.x * kSortTile;
-    const int lane = threadIdx.x & 63;
-    uint32_t v[kSortRounds], after[kSortRounds];  // after: the first id of the next 64
+    uint32_t v[kSortRounds];
 #pragma unroll
     for (int k = 0; k < kSortRounds; ++k) {
         const uint32_t i = base + k * 256 + threadIdx.x;
         v[k] = i < a.n ? sort_entry<FIRST>(a, i).x : ~0u;
-        if (FIRST) after[k] = lane == 63 && i + 1 < a.n ? a.ids.get(i + 1, a.V) : ~0u;
     }
+    if (FIRST && threadIdx.x == 0) id[kSortTile] = base + kSortTile < a.n ? a.ids.get(base + kSortTile, a.V) : ~0u;
     for (uint32_t b = threadIdx.x; b < bins; b += 256) h[b] = 0;
+    if (FIRST) {
+#pragma unroll
+        for (int k = 0; k < kSortRounds; ++k) id[k * 256 + threadIdx.x] = v[k];
+    }
     __syncthreads();
     int up = 1;
 #pragma unroll
-    for (int k = 0; k < kSortRounds; ++k) {
-        if (base + k * 256 + threadIdx.x < a.n) atomicAdd(&h[(v[k] >> a.shift) & (bins - 1)], 1u);
-        if (FIRST) {
-            const uint32_t next = __shfl_down(v[k], 1);
-            up &= v[k] <= (lane == 63 ? after[k] : next) || v[k] == ~0u;
+    for (int k = 0; k < kSortRounds; ++k)
+        if (v[k] != ~0u) {
+            atomicAdd(&h[(v[k] >> a.shift) & (bins - 1)], 1u);
+            if (FIRST) up &= v[k] <= id[k * 256 + threadIdx.x + 1];
         }
-    }
     up = __syncthreads_and(up);
     if (FIRST && threadIdx.x == 0) a.ascend[1 + blockIdx.x] = up;
     for (uint32_t b = threadIdx.x; b < bins; b += 256) a.hist[(size_t)blockIdx.x * bins + b] = h[b];
@@ -326,8 +353,8 @@ template <bool FIRST, typename I>
 __global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs<I> a, ZeroPart zeros) {
     __shared__ uint32_t cnt[4][1 << kSortBits];  // per wave: count, then where its entries of the digit go
     __shared__ uint32_t wsum[4];
-    if (blockIdx.x >= a.tiles) return store_zeros<256>(zeros, blockIdx.x - a.tiles, gridDim.x - a.tiles);
     if (*a.ascend) return;
+    if (blockIdx.x >= a.tiles) return store_zeros<256>(zeros, blockIdx.x - a.tiles, gridDim.x - a.tiles);
     const uint32_t bins = 1u << a.bits;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const uint32_t base = blockIdx.x * kSortTile + w * (kSortTile / 4);
@@ -406,11 +433,11 @@ struct SumArgs {
     int run;             // entries per subgroup
     uint32_t blocks;     // workgroups over the entries
     float *head, *tail;  // [blocks][D]: the sums of a workgroup's runs that began before it / go on after it
-    uint32_t rows;       // table form: entries per workgroup; few entries: rows per zeroing workgroup
+    uint32_t rows;       // table form: entries per workgroup; others: rows per zeroing workgroup
     uint8_t* named;      // table form: [blocks][V]
 };
 
-template <typename OT, int VEC, typename I>
+template <typename OT, int VEC, bool STREAM = false, typename I>
 __device__ __forceinline__ void put_row(const SumArgs<I>& a, uint32_t v, int64_t col, const float* acc) {
     OT* p = static_cast<OT*>(a.dw) + (int64_t)v * a.dwstride + col;
     Vec<OT, VEC> o;
@@ -422,7 +449,10 @@ __device__ __forceinline__ void put_row(const SumArgs<I>& a, uint32_t v, int64_t
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o.v[k] = (OT)(acc[k] * a.scale);
     }
-    store_vec<OT, VEC>(p, o);
+    if (STREAM)
+        stream_vec<OT, VEC>(p, o);
+    else
+        store_vec<OT, VEC>(p, o);
 }
 
 template <typename T, int VEC>
@@ -588,7 +618,8 @@ __global__ __launch_bounds__(1024) void embed_table_join_kernel(const SumArgs<I>
 }
 
 // ---- the general form: every subgroup walks `run` consecutive entries of the sorted list, and a
-// workgroup's 256 / lanes subgroups take consecutive pieces.  run: 16, or 8 where 16 would leave
+// workgroup's 256 / lanes subgroups take consecutive pieces.  Rows are stored past the caches: 500k ids
+// of rows of 32 floats take 56 us in all, 64 with cached stores.  run: 16, or 8 where 16 would leave
 // compute units without a workgroup.
 constexpr int kSumRun = 16;
 
@@ -647,7 +678,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs<I> a) {
                 part[head ? 0 : 1][tid] = o;
                 st |= head ? (goes_on ? 3 : 1) : 4;
             } else if (on) {
-                put_row<OT, VEC>(a, v, col, acc);
+                put_row<OT, VEC, true>(a, v, col, acc);
             }
             head = false;
 #pragma unroll
@@ -673,7 +704,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs<I> a) {
         if (open)
             keep(a.tail);
         else
-            put_row<OT, VEC>(a, key[e0 + a.run], col, acc);
+            put_row<OT, VEC, true>(a, key[e0 + a.run], col, acc);
     }
     if (s == 0 && (st & 1)) {  // the run that an earlier workgroup began
 #pragma unroll
@@ -681,6 +712,57 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs<I> a) {
         for (int q = 1; q < NS && (state[q - 1] & 2); ++q) add_vec<float, VEC>(acc, part[0][q * L + ln]);
         keep(a.head);
     }
+}
+
+// First entry whose id is at least v, of ids that ascend: 64 probes at a time, by a whole wave.
+template <typename I>
+__device__ __forceinline__ uint32_t first_at_least(const SumArgs<I>& a, uint32_t v) {
+    uint32_t lo = 0, hi = a.n;  // in [lo, hi]
+    const uint32_t lane = threadIdx.x & 63;
+    while (lo < hi) {
+        const uint32_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step - 1;
+        const uint32_t k = __popcll(__ballot(at < hi && a.ids.get(at, a.V) < v));  // these probes come first
+        hi = min(hi, lo + (k + 1) * step - 1);
+        lo += k * step;
+    }
+    return lo;
+}
+
+// The zeros of a table whose ids came in order, by workgroups of the joining launch: `rows` rows, those
+// that no id names.  (Nothing is then stored twice: a launch of the sort leaves the zeros out once it
+// knows.)
+template <typename OT, int VEC, typename I>
+__device__ __forceinline__ void zero_between(const SumArgs<I>& a, uint32_t r0) {
+    __shared__ uint8_t named[kFewRows];
+    __shared__ uint32_t range[2];
+    const int tid = threadIdx.x, w = tid >> 6, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
+    if (w < 2) {
+        const uint32_t e = first_at_least(a, min(a.V, r0 + w * a.rows));
+        if ((tid & 63) == 0) range[w] = e;
+    }
+    for (uint32_t k = tid; k < a.rows; k += 256) named[k] = 0;
+    __syncthreads();
+    const uint32_t e0 = range[0], e1 = range[1];
+    if (e1 - e0 <= 16 * a.rows) {
+        for (uint32_t e = e0 + tid; e < e1; e += 256) named[a.ids.get(e, a.V) - r0] = 1;
+    } else {  // rows that are named very often: one search per row
+        for (uint32_t k = tid; k < a.rows; k += 256) {
+            uint32_t lo = e0, hi = e1;
+            while (lo < hi) {
+                const uint32_t mid = lo + ((hi - lo) >> 1);
+                if (a.ids.get(mid, a.V) < r0 + k)
+                    lo = mid + 1;
+                else
+                    hi = mid;
+            }
+            named[k] = lo < e1 && a.ids.get(lo, a.V) == r0 + k;
+        }
+    }
+    __syncthreads();
+    const int64_t col = ((int64_t)blockIdx.y * L + ln) * VEC;
+    const float z[VEC] = {};
+    for (uint32_t k = s; k < a.rows && r0 + k < a.V; k += NS)
+        if (col < a.D && !named[k]) put_row<OT, VEC, true>(a, r0 + k, col, z);
 }
 
 // One workgroup per workgroup of the sums: if a run begins in it and goes on, its tail and the
@@ -691,10 +773,14 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const SumArgs<I> a) {
     __shared__ uint32_t s_last;
     const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
     const bool asc = a.ascend && *a.ascend;
+    if (blockIdx.x >= a.blocks) {
+        if (asc) zero_between<OT, VEC>(a, (blockIdx.x - a.blocks) * a.rows);
+        return;
+    }
     const uint32_t E = NS * a.run, b = blockIdx.x, i0 = b * E, i1 = i0 + E;
     if (i1 >= a.n) return;
-    const uint32_t v = sorted_id(a, asc, i1);
-    if (v >= a.V || sorted_id(a, asc, i1 - 1) != v || (b && sorted_id(a, asc, i0 - 1) == v)) return;
+    const uint32_t v = sorted_id(a, asc, i1), v1 = sorted_id(a, asc, i1 - 1), v0 = sorted_id(a, asc, b ? i0 - 1 : i1);
+    if (v >= a.V || v1 != v || (b && v0 == v)) return;
     if (tid < 64) {  // the last workgroup whose first entry is v's (the list is sorted): 64 probes at a time
         uint32_t lo = b + 1, hi = a.blocks;  // v's at lo, not at hi
         while (hi - lo > 1) {
@@ -790,50 +876,43 @@ static BwdPlan bwd_plan(int64_t V, int64_t n, int64_t D, int vec) {
     return p;
 }
 
-// the zeros of a dense gradient, in `parts` launches
-struct ZeroPlan {
-    char* base = nullptr;
-    int64_t units = 0;
-    ZeroPart edges{};
-    int parts = 1, next = 0;
-
-    ZeroPlan() = default;
-    ZeroPlan(void* dw, size_t bytes, int parts_) : parts(parts_) {
-        char *p = static_cast<char*>(dw), *end = p + bytes;
-        size_t before = (16 - (uintptr_t)p % 16) % 16;
-        if (before > bytes) before = bytes;
-        base = p + before;
-        units = (end - base) / 16;
-        edges.edge[0] = reinterpret_cast<uint16_t*>(p);
-        edges.nedge[0] = (int)before / 2;
-        edges.edge[1] = reinterpret_cast<uint16_t*>(base + units * 16);
-        edges.nedge[1] = (int)((end - base) % 16) / 2;
-    }
-    // the next launch's part and its workgroups
-    ZeroPart take(uint32_t& blocks) {
-        blocks = 0;
-        ZeroPart z{};
-        if (!base) return z;
-        if (next == 0) z = edges;
-        const int64_t u0 = units * next / parts, u1 = units * (next + 1) / parts;
-        z.p = reinterpret_cast<uint4*>(base) + u0;
-        z.units = u1 - u0;
-        blocks = (uint32_t)((z.units + kZeroUnits - 1) / kZeroUnits);
-        if (next == 0 && blocks == 0) blocks = 1;
-        ++next;
-        return z;
-    }
-};
+// the zeros of a dense gradient
+static ZeroPart all_zeros(void* dw, size_t bytes) {
+    ZeroPart z{};
+    char *p = static_cast<char*>(dw), *end = p + bytes;
+    size_t before = (16 - (uintptr_t)p % 16) % 16;
+    if (before > bytes) before = bytes;
+    z.p = reinterpret_cast<uint4*>(p + before);
+    z.units = (int64_t)(bytes - before) / 16;
+    z.edge[0] = reinterpret_cast<uint16_t*>(p);
+    z.nedge[0] = (int)before / 2;
+    z.edge[1] = reinterpret_cast<uint16_t*>(z.p + z.units);
+    z.nedge[1] = (int)(end - reinterpret_cast<char*>(z.p + z.units)) / 2;
+    return z;
+}
+// part k of `parts`, and its workgroups (none of a sum that is added to a table: z.p is null)
+static ZeroPart take_zeros(const ZeroPart& z, int k, int parts, uint32_t& blocks) {
+    blocks = 0;
+    if (!z.p) return z;
+    ZeroPart part = z;
+    const int64_t u0 = z.units * k / parts, u1 = z.units * (k + 1) / parts;
+    part.p = z.p + u0;
+    part.units = u1 - u0;
+    if (k) part.nedge[0] = part.nedge[1] = 0;
+    blocks = (uint32_t)((part.units + kZeroUnits - 1) / kZeroUnits);
+    if (k == 0 && blocks == 0) blocks = 1;
+    return part;
+}
 
 // sorts the ids: a.list, or a.ascend where they may turn out to be sorted
 template <typename I>
-static void launch_sort(const BwdPlan& p, char* w, SumArgs<I>& a, ZeroPlan zeros, hipStream_t s) {
+static void launch_sort(const BwdPlan& p, char* w, SumArgs<I>& a, const ZeroPart& z, hipStream_t s) {
     uint2 *la = reinterpret_cast<uint2*>(w + p.list_a), *lb = reinterpret_cast<uint2*>(w + p.list_b);
-    uint32_t zb;
+    uint32_t zb, zb1;
     if (p.form == kBucket) {
-        const ZeroPart z = zeros.take(zb);
+        const ZeroPart all = take_zeros(z, 0, 1, zb);
         hipLaunchKernelGGL((sort_bucket_kernel<I>), dim3(p.buckets + zb), dim3(1024), 0, s, a.n, a.ids, a.V, p.shift,
-                           p.passes, p.bits, la, p.buckets, z);
+                           p.passes, p.bits, la, p.buckets, all);
         a.list = la;
         return;
     }
@@ -847,23 +926,24 @@ static void launch_sort(const BwdPlan& p, char* w, SumArgs<I>& a, ZeroPlan zeros
     t.total = reinterpret_cast<uint32_t*>(w + p.total);
     t.ascend = reinterpret_cast<uint32_t*>(w + p.ascend);
     const unsigned scan_blocks = ((1u << p.bits) + 63) / 64;
+    const int parts = 2 * p.passes - 1;
     for (int pass = 0; pass < p.passes; ++pass) {
         t.in = pass == 0 ? nullptr : pass & 1 ? la : lb;
         t.out = pass & 1 ? lb : la;
         t.shift = pass * p.bits;
-        const ZeroPart z0 = zeros.take(zb);
+        // zeros from the first scatter on, where it is known whether the ids ascend
+        ZeroPart z0{};
+        if (pass) z0 = take_zeros(z, 2 * pass - 1, parts, zb);
+        const ZeroPart z1 = take_zeros(z, 2 * pass, parts, zb1);
         if (pass == 0) {
-            hipLaunchKernelGGL((sort_count_kernel<true, I>), dim3(p.tiles + zb), dim3(256), 0, s, t, z0);
+            hipLaunchKernelGGL((sort_count_kernel<true, I>), dim3(p.tiles), dim3(256), 0, s, t, z0);
             hipLaunchKernelGGL((sort_scan_kernel<true, I>), dim3(scan_blocks + 1), dim3(1024), 0, s, t);
+            hipLaunchKernelGGL((sort_scatter_kernel<true, I>), dim3(p.tiles + zb1), dim3(256), 0, s, t, z1);
         } else {
             hipLaunchKernelGGL((sort_count_kernel<false, I>), dim3(p.tiles + zb), dim3(256), 0, s, t, z0);
             hipLaunchKernelGGL((sort_scan_kernel<false, I>), dim3(scan_blocks), dim3(1024), 0, s, t);
+            hipLaunchKernelGGL((sort_scatter_kernel<false, I>), dim3(p.tiles + zb1), dim3(256), 0, s, t, z1);
         }
-        const ZeroPart z1 = zeros.take(zb);
-        if (pass == 0)
-            hipLaunchKernelGGL((sort_scatter_kernel<true, I>), dim3(p.tiles + zb), dim3(256), 0, s, t, z1);
-        else
-            hipLaunchKernelGGL((sort_scatter_kernel<false, I>), dim3(p.tiles + zb), dim3(256), 0, s, t, z1);
     }
     a.list = t.out;
     a.ascend = t.ascend;
@@ -885,8 +965,9 @@ static void launch_sums(const BwdPlan& p, const SumArgs<I>& a, uint32_t zero_blo
         default:
             hipLaunchKernelGGL((embed_sum_kernel<GT, OT, I, VEC>), dim3(a.blocks, p.slabs), block,
                                (2 * (256 / a.lanes) * a.run + 2) * sizeof(uint32_t), s, a);
-            if (a.blocks > 1)
-                hipLaunchKernelGGL((embed_join_kernel<OT, I, VEC>), dim3(a.blocks, p.slabs), block, 0, s, a);
+            if (a.blocks + zero_blocks > 1)
+                hipLaunchKernelGGL((embed_join_kernel<OT, I, VEC>), dim3(a.blocks + zero_blocks, p.slabs), block, 0, s,
+                                   a);
     }
 }
 
@@ -915,15 +996,13 @@ static int launch_bwd(const BwdPlan& p, char* w, SumArgs<I> a, const void* ids, 
     KernelTimer kt("embed_bwd", s);
     uint32_t zero_blocks = 0;
     const size_t dw_bytes = (size_t)a.V * a.D * elem_size(dwtype);
-    if (p.form == kFew && !a.accumulate) {  // about 32 KB of zeros per workgroup
+    if ((p.form == kFew || p.form == kRadix) && !a.accumulate) {  // about 32 KB of zeros per workgroup
         const int64_t rows = 32768 / ((int64_t)p.lanes * vec * elem_size(dwtype));
         a.rows = (uint32_t)(rows < 1 ? 1 : rows > kFewRows ? kFewRows : rows);
         zero_blocks = (a.V + a.rows - 1) / a.rows;
-    } else if (p.form == kBucket || p.form == kRadix) {
-        ZeroPlan zeros;
-        if (!a.accumulate) zeros = ZeroPlan(a.dw, dw_bytes, p.form == kBucket ? 1 : 2 * p.passes);
-        launch_sort(p, w, a, zeros, s);
     }
+    if (p.form == kBucket || p.form == kRadix)
+        launch_sort(p, w, a, a.accumulate ? ZeroPart{} : all_zeros(a.dw, dw_bytes), s);
     if (gtype == HGSR_F32)
         launch_sums<float>(dwtype, vec, p, a, zero_blocks, s);
     else if (gtype == HGSR_F16)
@@ -941,18 +1020,23 @@ struct FwdArgs {
     void* out;
 };
 
-template <typename WT, typename OT, typename I, int VEC>
+template <typename WT, typename OT, typename I, int VEC, bool STREAM>
 static void launch_fwd(const FwdArgs& a, hipStream_t s) {
     const uint32_t per_row = (uint32_t)(a.D / VEC);
     const RowIds<I> ids{static_cast<const I*>(a.ids), a.ids_stride};
     const int64_t most = ((int64_t)1 << 30) / per_row;  // rows per launch: at most 2^30 pieces
     for (int64_t r0 = 0; r0 < a.n; r0 += most) {
         const uint32_t chunks = (uint32_t)((a.n - r0 < most ? a.n - r0 : most) * per_row);
-        hipLaunchKernelGGL((embed_fwd_kernel<WT, OT, I, VEC>), dim3((chunks + 255) / 256), dim3(256), 0, s, chunks,
+        hipLaunchKernelGGL((embed_fwd_kernel<WT, OT, I, VEC, STREAM>), dim3((chunks + 255) / 256), dim3(256), 0, s, chunks,
                            fast_div(per_row), (uint32_t)a.V, static_cast<const WT*>(a.w),
-                           a.wstride, ids, r0, a.scale, static_cast<OT*>(a.out),
-                           stream_out(a.n * a.D * (int64_t)sizeof(OT)));
+                           a.wstride, ids, r0, a.scale, static_cast<OT*>(a.out));
     }
+}
+
+template <typename WT, typename OT, typename I, int VEC>
+static void launch_fwd(const FwdArgs& a, hipStream_t s) {
+    return stream_out(a.n * a.D * (int64_t)sizeof(OT)) ? launch_fwd<WT, OT, I, VEC, true>(a, s)
+                                                       : launch_fwd<WT, OT, I, VEC, false>(a, s);
 }
 
 template <typename WT, typename OT, typename I>
@@ -1039,8 +1123,7 @@ extern "C" int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, in
     if (n == 0) {
         if (!accumulate) {
             uint32_t zb;
-            ZeroPlan zeros(dw, dw_bytes, 1);
-            const ZeroPart z = zeros.take(zb);
+            const ZeroPart z = take_zeros(all_zeros(dw, dw_bytes), 0, 1, zb);
             hipLaunchKernelGGL(zero_kernel, dim3(zb), dim3(256), 0, s, z);
         }
         return check_launch("embed_bwd");

@@ -24,8 +24,8 @@ struct CacheArgs {
     RowIds<I> slots;                   // slots.p == nullptr: slot i
     void* x;                           // rows written, or the rows that a read fills
     int64_t xstride;
-    int stream;                        // read: the rows are stored past the caches
-    const int32_t* last;               // write: the last row of each named slot (nullable)
+    const int32_t* last;               // write: the last row of each named slot (nullable), unless
+    const uint32_t* distinct;          // this is set: no slot is named twice
 };
 
 template <typename I>
@@ -71,103 +71,125 @@ __device__ __forceinline__ void decode4(uint32_t w, float* o) {
 
 // ------------------------------------------------------------------------------------- write
 
-// the last row that names each slot: cleared where it will be read, then the largest row number
+// More than kFewSlots rows: the last row that names each slot, `last`, is cleared where it will be read
+// and then raised to the largest row number.  Slots in strictly ascending order (a compacted index,
+// a chunk appended) cannot repeat: the first launch finds out tile by tile, the second ends at
+// once, and the write does not look.
+constexpr int kSlotTile = 1024;
+struct SlotWork {
+    uint32_t* distinct;  // [1 + tiles]: the verdict, then the tiles' own
+    int32_t* last;       // [capacity]
+    uint32_t tiles;
+};
+
 template <typename I>
-__global__ __launch_bounds__(256) void slot_clear_kernel(uint32_t n, RowIds<I> slots, uint32_t capacity,
-                                                         int32_t* __restrict__ last) {
-    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const uint32_t c = slots.get(i, capacity);
-    if (c < capacity) last[c] = -1;
+__global__ __launch_bounds__(256) void slot_clear_kernel(uint32_t n, RowIds<I> slots, uint32_t capacity, SlotWork w) {
+    __shared__ uint32_t s[kSlotTile + 1];
+    const uint32_t base = blockIdx.x * kSlotTile;
+    uint32_t c[kSlotTile / 256];
+#pragma unroll
+    for (int k = 0; k < kSlotTile / 256; ++k) {
+        const uint32_t i = base + k * 256 + threadIdx.x;
+        c[k] = i < n ? slots.get(i, capacity) : ~0u;
+    }
+    const uint32_t end = base + kSlotTile;
+    if (threadIdx.x == 0) s[kSlotTile] = end < n ? slots.get(end, capacity) : ~0u;
+#pragma unroll
+    for (int k = 0; k < kSlotTile / 256; ++k) {
+        s[k * 256 + threadIdx.x] = c[k];
+        if (c[k] < capacity) w.last[c[k]] = -1;
+    }
+    __syncthreads();
+    int up = 1;
+#pragma unroll
+    for (int k = 0; k < kSlotTile / 256; ++k) up &= c[k] < s[k * 256 + threadIdx.x + 1] || c[k] == ~0u;
+    up = __syncthreads_and(up);
+    if (threadIdx.x == 0) w.distinct[1 + blockIdx.x] = up;
 }
 template <typename I>
-__global__ __launch_bounds__(256) void slot_last_kernel(uint32_t n, RowIds<I> slots, uint32_t capacity,
-                                                        int32_t* __restrict__ last) {
-    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const uint32_t c = slots.get(i, capacity);
-    if (c < capacity) atomicMax(&last[c], (int32_t)i);
+__global__ __launch_bounds__(256) void slot_last_kernel(uint32_t n, RowIds<I> slots, uint32_t capacity, SlotWork w) {
+    int up = 1;
+    for (uint32_t t = threadIdx.x; t < w.tiles; t += 256) up &= w.distinct[1 + t];
+    up = __syncthreads_and(up);
+    if (blockIdx.x == 0 && threadIdx.x == 0) w.distinct[0] = up;
+    if (up) return;
+#pragma unroll
+    for (int k = 0; k < kSlotTile / 256; ++k) {
+        const uint32_t i = blockIdx.x * kSlotTile + k * 256 + threadIdx.x, c = i < n ? slots.get(i, capacity) : capacity;
+        if (c < capacity) atomicMax(&w.last[c], (int32_t)i);
+    }
 }
 
 // VEC consecutive columns per lane; ALIGNED: whole pieces, moved as vectors.  FEW: no more than
 // kFewSlots rows, whose repeated slots are found here, by a group's lanes among the later rows.
 constexpr int kFewSlots = 1024;
-constexpr int kWritePer = 2;  // pieces per lane, 256 apart
 
 template <typename XT, typename I, int FMT, int VEC, bool ALIGNED, bool FEW>
 __global__ __launch_bounds__(256) void rowcache_write_kernel(const CacheArgs<I> a) {
     __shared__ uint32_t slots[FEW ? kFewSlots : 1];
-    const uint32_t c0 = xcd_remap(blockIdx.x, gridDim.x) * (256 * kWritePer) + threadIdx.x;
-    const int lanes = a.group / VEC;  // a power of two, <= 32
-    uint32_t slot[kWritePer], r[kWritePer];
-    int64_t col[kWritePer];
-    float x[kWritePer][VEC];
+    // an XCD's workgroups take consecutive rows: slots in order then share its L2's lines
+    const uint32_t c = xcd_remap(blockIdx.x, gridDim.x) * 256 + threadIdx.x;
+    const bool in = c < a.chunks;
+    const uint32_t r = a.per_row.div(in ? c : 0);
+    const int64_t row = a.row0 + r, col = in ? (int64_t)(c - r * a.per_row.d) * VEC : a.D;
+    const uint32_t slot = slot_of(a, row);
+    float x[VEC];
+    const XT* p = static_cast<const XT*>(a.x) + row * a.xstride + col;
+    if (ALIGNED) {
+        Vec<XT, VEC> v{};
+        if (col < a.D) v = load_vec<XT, VEC>(p);
 #pragma unroll
-    for (int q = 0; q < kWritePer; ++q) {
-        const uint32_t c = c0 + q * 256;
-        const bool in = c < a.chunks;
-        r[q] = a.per_row.div(in ? c : 0);
-        col[q] = in ? (int64_t)(c - r[q] * a.per_row.d) * VEC : a.D;
-        slot[q] = slot_of(a, a.row0 + r[q]);
-        const XT* p = static_cast<const XT*>(a.x) + (a.row0 + r[q]) * a.xstride + col[q];
-        if (ALIGNED) {
-            Vec<XT, VEC> v{};
-            if (col[q] < a.D) v = load_vec<XT, VEC>(p);
+        for (int k = 0; k < VEC; ++k) x[k] = (float)v.v[k];
+    } else {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) x[q][k] = (float)v.v[k];
-        } else {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) x[q][k] = col[q] + k < a.D ? (float)p[k] : 0.0f;
-        }
+        for (int k = 0; k < VEC; ++k) x[k] = col + k < a.D ? (float)p[k] : 0.0f;
     }
     if (FEW) {
-        const uint32_t n = (uint32_t)a.n;
-        for (uint32_t i = threadIdx.x; i < n; i += 256) slots[i] = slot_of(a, i);
+        for (uint32_t i = threadIdx.x; i < (uint32_t)a.n; i += 256) slots[i] = slot_of(a, i);
         __syncthreads();
     }
+    bool on = col < a.D && slot < a.capacity;
+    if (!FEW && a.last && !*a.distinct && on) on = a.last[slot] == (int32_t)row;
+    // the largest magnitude of the group as bits: infinities and NaN lie above every number
+    const int lanes = a.group / VEC;  // a power of two, <= 16
+    uint32_t m = 0;
 #pragma unroll
-    for (int q = 0; q < kWritePer; ++q) {
-        bool on = col[q] < a.D && slot[q] < a.capacity;
-        if (!FEW && a.last && on) on = a.last[slot[q]] == (int32_t)(a.row0 + r[q]);
-        // the largest magnitude of the group as bits: infinities and NaN lie above every number
-        uint32_t m = 0;
+    for (int k = 0; k < VEC; ++k) m = max(m, __float_as_uint(x[k]) & 0x7fffffffu);
+    if (FEW)  // a later row of the same slot: a mark above every magnitude
+        for (uint32_t j = (uint32_t)row + 1 + (threadIdx.x & (lanes - 1)); j < (uint32_t)a.n; j += lanes)
+            if (slots[j] == slot) m = 0x80000000u;
+    for (int d = 1; d < lanes; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+    if (!on || (FEW && m == 0x80000000u)) return;
+    const bool finite = m < 0x7f800000u;
+    const float per = FMT == HGSR_INT8 ? 1.0f / 127.0f : 1.0f / 448.0f;
+    const float s = fmaxf(__uint_as_float(m) * per, kScaleFloor), inv = 1.0f / s;
+    uint32_t w[VEC / 4];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) m = max(m, __float_as_uint(x[q][k]) & 0x7fffffffu);
-        if (FEW)  // a later row of the same slot: a mark above every magnitude
-            for (uint32_t j = (uint32_t)a.row0 + r[q] + 1 + (threadIdx.x & (lanes - 1)); j < (uint32_t)a.n; j += lanes)
-                if (slots[j] == slot[q]) m = 0x80000000u;
-        for (int d = 1; d < lanes; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
-        if (!on || (FEW && m == 0x80000000u)) continue;
-        const bool finite = m < 0x7f800000u;
-        const float per = FMT == HGSR_INT8 ? 1.0f / 127.0f : 1.0f / 448.0f;
-        const float s = fmaxf(__uint_as_float(m) * per, kScaleFloor), inv = 1.0f / s;
-        uint32_t w[VEC / 4];
+    for (int k = 0; k < VEC; k += 4) {
+        float y[4];
 #pragma unroll
-        for (int k = 0; k < VEC; k += 4) {
-            float y[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = finite ? quotient_odd(x[q][k + j], s, inv) : 0.0f;
-            w[k / 4] = encode4<FMT>(y[0], y[1], y[2], y[3]);
-        }
-        uint8_t* to = a.codes + (int64_t)slot[q] * a.cstride + col[q];
-        if (ALIGNED) {
-            Vec<uint32_t, VEC / 4> o;
-#pragma unroll
-            for (int k = 0; k < VEC / 4; ++k) o.v[k] = w[k];
-            store_vec<uint32_t, VEC / 4>(reinterpret_cast<uint32_t*>(to), o);
-        } else {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k)
-                if (col[q] + k < a.D) to[k] = (uint8_t)(w[k / 4] >> (8 * (k & 3)));
-        }
-        if ((col[q] & (a.group - 1)) == 0)
-            a.scales[(int64_t)slot[q] * a.sstride + (col[q] >> a.glog)] = finite ? s : __builtin_nanf("");
+        for (int j = 0; j < 4; ++j) y[j] = finite ? quotient_odd(x[k + j], s, inv) : 0.0f;
+        w[k / 4] = encode4<FMT>(y[0], y[1], y[2], y[3]);
     }
+    uint8_t* to = a.codes + (int64_t)slot * a.cstride + col;
+    if (ALIGNED) {
+        Vec<uint32_t, VEC / 4> o;
+#pragma unroll
+        for (int k = 0; k < VEC / 4; ++k) o.v[k] = w[k];
+        store_vec<uint32_t, VEC / 4>(reinterpret_cast<uint32_t*>(to), o);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            if (col + k < a.D) to[k] = (uint8_t)(w[k / 4] >> (8 * (k & 3)));
+    }
+    if ((col & (a.group - 1)) == 0)
+        a.scales[(int64_t)slot * a.sstride + (col >> a.glog)] = finite ? s : __builtin_nanf("");
 }
 
 // -------------------------------------------------------------------------------------- read
 
-template <typename OT, typename I, int FMT, int VEC, bool ALIGNED>
+// STREAM: the rows are stored past the caches
+template <typename OT, typename I, int FMT, int VEC, bool ALIGNED, bool STREAM>
 __global__ __launch_bounds__(256) void rowcache_read_kernel(const CacheArgs<I> a) {
     const uint32_t c = blockIdx.x * 256 + threadIdx.x;
     if (c >= a.chunks) return;
@@ -200,7 +222,7 @@ __global__ __launch_bounds__(256) void rowcache_read_kernel(const CacheArgs<I> a
         Vec<OT, VEC> o;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o.v[k] = (OT)x[k];
-        if (a.stream)
+        if (STREAM)
             stream_vec<OT, VEC>(to, o);
         else
             store_vec<OT, VEC>(to, o);
@@ -215,13 +237,15 @@ __global__ __launch_bounds__(256) void rowcache_read_kernel(const CacheArgs<I> a
 
 template <typename T, int FMT, int VEC, bool ALIGNED, typename I>
 static void launch(bool write, const CacheArgs<I>& a, hipStream_t s) {
-    const dim3 block(256), wgrid((a.chunks + 256 * kWritePer - 1) / (256 * kWritePer)), rgrid((a.chunks + 255) / 256);
-    if (!write)
-        hipLaunchKernelGGL((rowcache_read_kernel<T, I, FMT, VEC, ALIGNED>), rgrid, block, 0, s, a);
+    const dim3 block(256), grid((a.chunks + 255) / 256);
+    if (!write && ALIGNED && stream_out(a.n * a.D * (int64_t)sizeof(T)))
+        hipLaunchKernelGGL((rowcache_read_kernel<T, I, FMT, VEC, ALIGNED, ALIGNED>), grid, block, 0, s, a);
+    else if (!write)
+        hipLaunchKernelGGL((rowcache_read_kernel<T, I, FMT, VEC, ALIGNED, false>), grid, block, 0, s, a);
     else if (a.slots.p && a.n > 1 && a.n <= kFewSlots)
-        hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, ALIGNED, true>), wgrid, block, 0, s, a);
+        hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, ALIGNED, true>), grid, block, 0, s, a);
     else
-        hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, ALIGNED, false>), wgrid, block, 0, s, a);
+        hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, ALIGNED, false>), grid, block, 0, s, a);
 }
 
 template <typename T, int FMT, int VEC, typename I>
@@ -255,6 +279,14 @@ struct CacheCall {
     float* scales;
 };
 
+static SlotWork slot_work(void* ws, int64_t n) {
+    SlotWork w;
+    w.tiles = (uint32_t)((n + kSlotTile - 1) / kSlotTile);
+    w.distinct = static_cast<uint32_t*>(ws);
+    w.last = reinterpret_cast<int32_t*>(static_cast<char*>(ws) + align256(((size_t)w.tiles + 1) * 4));
+    return w;
+}
+
 template <typename I>
 static void launch(bool write, const CacheCall& c, hipStream_t s) {
     CacheArgs<I> a{};
@@ -270,15 +302,18 @@ static void launch(bool write, const CacheCall& c, hipStream_t s) {
     a.slots = RowIds<I>{static_cast<const I*>(c.slots), c.slots_stride};
     a.x = c.x;
     a.xstride = c.xstride;
-    a.stream = stream_out(c.n * c.D * elem_size(c.type));
     if (write && c.slots && c.n > kFewSlots) {
-        int32_t* last = static_cast<int32_t*>(c.ws);
-        const dim3 grid((unsigned)((c.n + 255) / 256));
-        hipLaunchKernelGGL((slot_clear_kernel<I>), grid, dim3(256), 0, s, (uint32_t)c.n, a.slots, a.capacity, last);
-        hipLaunchKernelGGL((slot_last_kernel<I>), grid, dim3(256), 0, s, (uint32_t)c.n, a.slots, a.capacity, last);
-        a.last = last;
+        const SlotWork w = slot_work(c.ws, c.n);
+        hipLaunchKernelGGL((slot_clear_kernel<I>), dim3(w.tiles), dim3(256), 0, s, (uint32_t)c.n, a.slots, a.capacity, w);
+        hipLaunchKernelGGL((slot_last_kernel<I>), dim3(w.tiles), dim3(256), 0, s, (uint32_t)c.n, a.slots, a.capacity, w);
+        a.last = w.last;
+        a.distinct = w.distinct;
     }
-    if (c.type == HGSR_F32)
+    // f32 rows: a write moves 8 columns per lane (27.3 us for 500k rows of 32; 34.3 with 4), a read 4 (16.8
+    // us; 18.6 with 8: its 16-byte stores would be 32 bytes apart)
+    if (c.type == HGSR_F32 && write)
+        launch<float, 8>(write, c.format, a, s);
+    else if (c.type == HGSR_F32)
         launch<float, 4>(write, c.format, a, s);
     else if (c.type == HGSR_F16)
         launch<f16_t, 8>(write, c.format, a, s);
@@ -311,7 +346,8 @@ static int check_cache(const char* what, const CacheCall& c) {
 }
 
 extern "C" size_t hgsr_rowcache_write_ws_bytes(int64_t capacity, int64_t n, int has_slots) {
-    return has_slots && n > kFewSlots && capacity > 0 ? (size_t)capacity * sizeof(int32_t) : 0;
+    if (!has_slots || n <= kFewSlots || capacity <= 0) return 0;
+    return align256(((size_t)(n + kSlotTile - 1) / kSlotTile + 1) * 4) + (size_t)capacity * sizeof(int32_t);
 }
 
 extern "C" int hgsr_rowcache_write(int64_t capacity, int64_t n, int64_t D, int group, int format, const void* x,

@@ -95,7 +95,7 @@ def _grad(grad, flat, out, scale, accumulate, index):
     ws = torch.empty(ws_b, dtype=torch.uint8, device=out.device) if ws_b else None
     N.call_on(index, "hgsr_embed_bwd", V, n, D, grad.data_ptr(), _TYPES[grad.dtype], row_stride(grad, "grad"),
               flat.data_ptr(), _IDS[flat.dtype], id_stride(flat), scale, out.data_ptr(), _TYPES[out.dtype],
-              row_stride(out, "out"), int(accumulate), ws.data_ptr() if ws_b else None, ws_b)
+              row_stride(out, "out"), accumulate, ws.data_ptr() if ws_b else None, ws_b)
     return out
 
 
@@ -103,19 +103,19 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, flat, shape, scale, dtype, index):
         ctx.save_for_backward(flat)
-        ctx.args = (weight.shape, weight.dtype, gradbuf.key(weight), scale, index)
+        ctx.args = weight.shape, weight.dtype, (weight.data_ptr(), weight.numel()), scale, index
         return _lookup(weight, flat, shape, scale, dtype, index)
 
     @staticmethod
     def backward(ctx, g):
-        (flat,) = ctx.saved_tensors
+        flat, = ctx.saved_tensors
         shape, dtype, key, scale, index = ctx.args
         if torch.is_grad_enabled():  # create_graph: the gradient is linear in g, and its own gradient a lookup
             return _EmbeddingGrad.apply(g, flat, shape, dtype, scale, index), None, None, None, None, None
         out = gradbuf.take(key, shape, dtype)  # in place in a DDP bucket when one is registered
         if out is None:
             out = g.new_empty(shape, dtype=dtype)
-        return _grad(rows_view(g, shape[1], "grad"), flat, out, scale, False, index), None, None, None, None, None
+        return _grad(rows_view(g, shape[1], "grad"), flat, out, scale, 0, index), None, None, None, None, None
 
 
 class _EmbeddingGrad(torch.autograd.Function):
@@ -123,7 +123,7 @@ class _EmbeddingGrad(torch.autograd.Function):
     def forward(ctx, g, flat, shape, dtype, scale, index):
         ctx.save_for_backward(flat)
         ctx.args = (g.shape, g.dtype, scale, index)
-        return _grad(rows_view(g, shape[1], "grad"), flat, g.new_empty(shape, dtype=dtype), scale, False, index)
+        return _grad(rows_view(g, shape[1], "grad"), flat, g.new_empty(shape, dtype=dtype), scale, 0, index)
 
     @staticmethod
     def backward(ctx, gg):
@@ -174,7 +174,7 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
         dtype = grad.dtype if dtype is None else dtype
         type_code(dtype)
         index = check_device(grad, ids)
-        out, accumulate = grad.new_empty((num_rows, D), dtype=dtype), False
+        out, accumulate = grad.new_empty((num_rows, D), dtype=dtype), 0
     else:
         type_code(out.dtype)
         if tuple(out.shape) != (num_rows, D) or (dtype is not None and dtype != out.dtype):
@@ -182,7 +182,7 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
                              f"{dtype or 'its type'}")
         if row_stride(out, "out") < D:
             raise ValueError("hgsr: the rows of out overlap")
-        index, accumulate = check_device(grad, ids, out), True
+        index, accumulate = check_device(grad, ids, out), 1
     g = rows_view(grad, D, "grad") if D else grad
     return _grad(g, flat_ids(ids), out, float(scale), accumulate, index)
 

@@ -51,6 +51,8 @@ def alloc_key(k, like: torch.Tensor) -> torch.Tensor:
 def take(k, shape, dtype):
     """The registered destination (taken) of the tensor whose key is `k`, or None: for a backward
     that has neither the tensor nor one like it."""
+    if not _DEST:
+        return None
     d = _DEST.pop(k, None)
     return d if d is not None and tuple(d.shape) == tuple(shape) and d.dtype == dtype else None
 

@@ -41,6 +41,9 @@ def make_ids(kind, V, n, seed, dtype=torch.int64):
         ids = torch.randint(0, V, (n,), generator=g)
         far = torch.tensor([-1, V, -2 ** 31, 2 ** 31 - 1])[torch.randint(0, 4, (n,), generator=g)]
         ids = torch.where(torch.rand(n, generator=g) < 0.3, far, ids)
+    elif kind == "tail":  # in order, padding behind
+        ids = torch.randint(0, V, (n,), generator=g).sort().values
+        ids[n - n // 3:] = -1
     elif kind == "none":
         ids = torch.full((n,), -1)
     else:  # half of the entries one row, the rest spread
@@ -121,7 +124,9 @@ def test_grad(V, n, D, gt, ot):
     (5_000_000, 30_000, 1, "mixed"), (65_536, 40_000, 64, "mixed"), (3, 16_384, 256, "mixed"), (3, 16_385, 256, "mixed"),
     (70_000, 4096, 40, "padded"), (70_000, 4097, 40, "padded"), (2048, 1024, 640, "mixed"), (2047, 1025, 640, "mixed"),
     (300, 256, 2048, "one"), (300, 257, 2048, "one"), (1_000_000, 250_000, 32, "sorted"), (4096, 65_536, 5, "mixed"),
-    (2048, 100_000, 33, "reversed")])
+    (2048, 100_000, 33, "reversed"), (70_000, 40_000, 8, "one"), (2048, 100_000, 33, "sorted"),
+    (50_000, 30_000, 24, "tail"), (3000, 20_000, 8, "none"), (1_500_000, 17_000, 4, "tail"), (600, 9000, 48, "tail"),
+    (600, 16_384, 8, "one"), (1 << 20, 16_000, 8, "mixed"), (200, 5000, 100, "uniform")])
 def test_grad_of_whole_numbers_is_exact(V, n, D, kind):
     ids = make_ids(kind, V, n, n).to(DEV)
     g = torch.randint(-8, 9, (n, D), generator=gen(V)).to(DEV)

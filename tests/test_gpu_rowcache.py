@@ -176,6 +176,26 @@ def test_repeated_and_outside_slots(n):
     assert torch.equal(c.codes[cap - 1].cpu().double(), torch.from_numpy(want_write(x[-1:].numpy(), "int8", 32)[0])[0])
 
 
+@pytest.mark.parametrize("n", [1025, 2048, 2049, 30_000])
+@pytest.mark.parametrize("twice", [None, 0, 2047, -2])
+def test_slots_in_order(n, twice):
+    """Ascending slots, as a compacted index has them, with no slot or one slot named twice."""
+    cap = n + n // 2
+    slots = torch.randperm(cap, generator=gen(n))[:n].sort().values
+    if twice is not None and twice + 1 < n:
+        slots[twice + 1] = slots[twice]
+    x = torch.randn(n, 32, generator=gen(n + 1))
+    c = R.rowcache_alloc(cap, 32, "int8", 32, DEV)
+    R.rowcache_write(c, x.to(DEV), slots.to(DEV))
+    final = torch.zeros(cap, 32)
+    final[slots] = x  # the later of two equal slots
+    if twice is not None and twice + 1 < n:
+        final[slots[twice]] = x[twice + 1]
+    q, s = want_write(final[slots].numpy(), "int8", 32)
+    np.testing.assert_array_equal(c.codes[slots.to(DEV)].cpu().numpy(), q)
+    np.testing.assert_array_equal(c.scales[slots.to(DEV)].cpu().numpy(), s)
+
+
 def test_every_code_reads_as_its_value():
     for fmt in ("int8", "e4m3"):
         bits = torch.arange(256, dtype=torch.uint8)
