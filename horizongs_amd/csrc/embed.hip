@@ -101,66 +101,177 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {  // inclus
 
 // Up to kBucketMost entries: one launch.  The ids are cut into up to 256 ranges, a workgroup each: it
 // reads all ids, keeps the positions of its own in LDS (in order) and counts the smaller ones, which
-// is where its part of the list starts; then it sorts what it kept by the ids' remaining bits.
+// is where its part of the list starts; then it sorts what it kept by the ids' remaining bits.  A
+// range that does not fit (an id that half of the entries name) is sorted in global memory.
 // (One workgroup for all: 42 us at 16,384 entries, LDS-bound; counting, for each entry, the ones
-// before it: 36 us of the whole chip.)
-constexpr int kBucketMost = 16384;
-constexpr int kBucketRounds = kBucketMost / 1024;
+// before it: 36 us of the whole chip; this: 14.)
+constexpr int kBucketMost = 32768;
+constexpr int kBucketKeep = 8192;  // positions that a workgroup keeps
+constexpr int kBucketRounds = kBucketKeep / 1024;
 constexpr int kBucketLog = 8;
-constexpr int kBucketBits = 9;  // per pass
+constexpr int kBucketBits = 9;   // per pass
 constexpr int kCountMost = 512;  // entries that a workgroup sorts by counting
 
 template <typename I>
-__global__ __launch_bounds__(1024) void sort_bucket_kernel(uint32_t n, RowIds<I> ids, uint32_t V, int shift, int passes,
-                                                           int bits, uint2* __restrict__ out, uint32_t buckets,
-                                                           ZeroPart zeros) {
-    __shared__ uint16_t pos[kBucketMost];
+struct BucketArgs {
+    uint32_t n, V;
+    RowIds<I> ids;
+    int shift, passes, bits;
+    uint32_t buckets;
+    uint2 *out, *tmp;
+};
+
+// per wave and digit: counts -> where the wave's entries of the digit go (after all smaller digits and the
+// earlier waves'); 1024 threads
+__device__ __forceinline__ void digit_places(uint32_t (*cnt)[1 << kBucketBits], uint32_t* wsum, uint32_t bins) {
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+    uint32_t c[16], sum = 0;
+    if ((uint32_t)tid < bins) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) c[q] = cnt[q][tid];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) sum += c[q];
+    }
+    const uint32_t inc = wave_scan(sum, lane);
+    if (lane == 63) wsum[w] = inc;
+    __syncthreads();
+    uint32_t to = inc - sum;
+    for (int q = 0; q < w; ++q) to += wsum[q];
+    if ((uint32_t)tid < bins) {
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            cnt[q][tid] = to;
+            to += c[q];
+        }
+    }
+    __syncthreads();
+}
+
+// the wave's next entries that hold digit d: their places, one after the other
+__device__ __forceinline__ uint32_t take_places(uint32_t* cnt, uint32_t d, bool on, int bits, int lane) {
+    const uint64_t same = match<kBucketBits>(d, on, bits);
+    const int first = __ffsll((unsigned long long)same) - 1;
+    uint32_t old = 0;
+    if (on && lane == first) old = atomicAdd(&cnt[d], (uint32_t)__popcll(same));
+    return __shfl(old, first) + __popcll(same & below(lane));
+}
+
+template <typename I>
+__global__ __launch_bounds__(1024) void sort_bucket_kernel(const BucketArgs<I> a, ZeroPart zeros) {
+    __shared__ uint16_t pos[kBucketKeep];
     __shared__ __align__(16) uint32_t cnt[16][1 << kBucketBits];
     __shared__ uint32_t wsum[2][16];
-    if (blockIdx.x >= buckets) return store_zeros<1024>(zeros, blockIdx.x - buckets, gridDim.x - buckets);
+    if (blockIdx.x >= a.buckets) return store_zeros<1024>(zeros, blockIdx.x - a.buckets, gridDim.x - a.buckets);
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-    int rounds = (n + 1023) / 1024;
-    uint32_t base = w * rounds * 64 + lane;  // a wave's entries are consecutive
-    uint32_t k[kBucketRounds], place[kBucketRounds];
-    uint16_t p[kBucketRounds];
+    const uint32_t bucket = blockIdx.x, n = a.n, bins = 1u << a.bits;
+    uint32_t m = 0, start = 0;
+    for (uint32_t j0 = 0; j0 < n; j0 += kBucketKeep) {  // a wave's entries are consecutive
+        const int rounds = (int)((min(n - j0, (uint32_t)kBucketKeep) + 1023) / 1024);
+        const uint32_t base = j0 + w * rounds * 64 + lane;
+        uint32_t k[kBucketRounds], mine = 0, less = 0;
 #pragma unroll
-    for (int r = 0; r < kBucketRounds; ++r)
-        if (r < rounds) k[r] = base + r * 64 < n ? ids.get(base + r * 64, V) : ~0u;
-    uint32_t mine = 0, less = 0;
+        for (int r = 0; r < kBucketRounds; ++r)
+            if (r < rounds) k[r] = base + r * 64 < n ? a.ids.get(base + r * 64, a.V) : ~0u;
 #pragma unroll
-    for (int r = 0; r < kBucketRounds; ++r)
-        if (r < rounds) {
-            mine += __popcll(__ballot(k[r] >> shift == blockIdx.x && k[r] != ~0u));
-            less += __popcll(__ballot(k[r] >> shift < blockIdx.x));
+        for (int r = 0; r < kBucketRounds; ++r)
+            if (r < rounds) {
+                mine += __popcll(__ballot(k[r] >> a.shift == bucket && k[r] != ~0u));
+                less += __popcll(__ballot(k[r] >> a.shift < bucket));
+            }
+        if (lane == 0) {
+            wsum[0][w] = mine;
+            wsum[1][w] = less;
         }
-    if (lane == 0) {
-        wsum[0][w] = mine;
-        wsum[1][w] = less;
-    }
-    __syncthreads();
-    uint32_t m = 0, start = 0, at = 0;
+        __syncthreads();
+        uint32_t at = m;
 #pragma unroll
-    for (int q = 0; q < 16; ++q) {
-        if (q < w) at += wsum[0][q];
-        m += wsum[0][q];
-        start += wsum[1][q];
+        for (int q = 0; q < 16; ++q) {
+            if (q < w) at += wsum[0][q];
+            m += wsum[0][q];
+            start += wsum[1][q];
+        }
+#pragma unroll
+        for (int r = 0; r < kBucketRounds; ++r)
+            if (r < rounds) {
+                const bool in = k[r] >> a.shift == bucket && k[r] != ~0u;
+                const uint64_t b = __ballot(in);
+                const uint32_t to = at + __popcll(b & below(lane));
+                if (in && to < kBucketKeep) pos[to] = (uint16_t)(base + r * 64);
+                at += __popcll(b);
+            }
+        __syncthreads();
     }
     if (m == 0) return;
-#pragma unroll
-    for (int r = 0; r < kBucketRounds; ++r)
-        if (r < rounds) {
-            const bool in = k[r] >> shift == blockIdx.x && k[r] != ~0u;
+    uint2 *out = a.out + start, *tmp = a.tmp + start;
+    if (m > kBucketKeep) {
+        // the range once more, its entries into global memory in order: done if they are one id's
+        uint2* src = a.passes & 1 ? tmp : out;
+        uint32_t filled = 0, lowest = ~0u, highest = 0;
+        for (uint32_t j0 = 0; j0 < n; j0 += 1024) {
+            const uint32_t i = j0 + tid, k = i < n ? a.ids.get(i, a.V) : ~0u;
+            const bool in = k != ~0u && k >> a.shift == bucket;
             const uint64_t b = __ballot(in);
-            if (in) pos[at + __popcll(b & below(lane))] = (uint16_t)(base + r * 64);
-            at += __popcll(b);
+            if (lane == 0) wsum[0][w] = __popcll(b);
+            __syncthreads();
+            uint32_t at = filled + __popcll(b & below(lane));
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                if (q < w) at += wsum[0][q];
+                filled += wsum[0][q];
+            }
+            if (in) {
+                src[at] = make_uint2(k, i);
+                lowest = min(lowest, k);
+                highest = max(highest, k);
+            }
+            __syncthreads();
         }
-    __syncthreads();
-    out += start;
-    rounds = (m + 1023) / 1024;
-    base = w * rounds * 64 + lane;
-    if (passes == 0) {  // a range of one id
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            lowest = min(lowest, (uint32_t)__shfl_xor((int)lowest, d));
+            highest = max(highest, (uint32_t)__shfl_xor((int)highest, d));
+        }
+        if (lane == 0) {
+            wsum[0][w] = lowest;
+            wsum[1][w] = highest;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            lowest = min(lowest, wsum[0][q]);
+            highest = max(highest, wsum[1][q]);
+        }
+        __syncthreads();
+        const uint32_t share = (m + 1023) / 1024 * 64, i0 = w * share, i1 = min(m, i0 + share);
+        if (lowest == highest) {
+            if (src == tmp)
+                for (uint32_t i = tid; i < m; i += 1024) out[i] = tmp[i];
+            return;
+        }
+        for (int pass = 0; pass < a.passes; ++pass) {
+            const int sh = pass * a.bits;
+            uint2* dst = src == out ? tmp : out;
+            for (uint32_t b = tid; b < 16 * bins; b += 1024) cnt[b >> a.bits][b & (bins - 1)] = 0;
+            __syncthreads();
+            for (uint32_t i = i0 + lane; i < i1; i += 64) atomicAdd(&cnt[w][(src[i].x >> sh) & (bins - 1)], 1u);
+            __syncthreads();
+            digit_places(cnt, wsum[0], bins);
+            for (uint32_t i = i0; i < i1; i += 64) {
+                const bool on = i + lane < i1;
+                const uint2 e = src[on ? i + lane : i];
+                const uint32_t to = take_places(cnt[w], (e.x >> sh) & (bins - 1), on, a.bits, lane);
+                if (on) dst[to] = e;
+            }
+            __syncthreads();
+            src = dst;
+        }
+        return;
+    }
+    const int rounds = (m + 1023) / 1024;
+    const uint32_t base = w * rounds * 64 + lane;
+    if (a.passes == 0) {  // a range of one id
         for (int r = 0; r < rounds; ++r)
-            if (base + r * 64 < m) out[base + r * 64] = make_uint2(blockIdx.x, pos[base + r * 64]);
+            if (base + r * 64 < m) out[base + r * 64] = make_uint2(bucket, pos[base + r * 64]);
         return;
     }
     if (m <= kCountMost) {
@@ -169,7 +280,7 @@ __global__ __launch_bounds__(1024) void sort_bucket_kernel(uint32_t n, RowIds<I>
         uint32_t *id = cnt[0], *before = cnt[0] + kCountMost;
         const uint32_t width = m <= 64 ? 64 : m <= 128 ? 128 : m <= 256 ? 256 : 512, parts = 1024 / width;
         if ((uint32_t)tid < width) {
-            id[tid] = (uint32_t)tid < m ? ids.get(pos[tid], V) : ~0u;
+            id[tid] = (uint32_t)tid < m ? a.ids.get(pos[tid], a.V) : ~0u;
             before[tid] = 0;
         }
         __syncthreads();
@@ -187,59 +298,32 @@ __global__ __launch_bounds__(1024) void sort_bucket_kernel(uint32_t n, RowIds<I>
         if ((uint32_t)tid < m) out[before[tid]] = make_uint2(own, pos[tid]);
         return;
     }
-    const uint32_t bins = 1u << bits;
-    for (int pass = 0; pass < passes; ++pass) {
-        const int sh = pass * bits;
+    uint32_t k[kBucketRounds], place[kBucketRounds];
+    uint16_t p[kBucketRounds];
+    for (int pass = 0; pass < a.passes; ++pass) {
+        const int sh = pass * a.bits;
 #pragma unroll
         for (int r = 0; r < kBucketRounds; ++r)
             if (r < rounds) {
-                const bool on = base + r * 64 < m;
-                p[r] = on ? pos[base + r * 64] : 0;
-                k[r] = ids.get(p[r], V);
+                p[r] = base + r * 64 < m ? pos[base + r * 64] : 0;
+                k[r] = a.ids.get(p[r], a.V);
             }
-        for (uint32_t b = tid; b < 16 * bins; b += 1024) cnt[b >> bits][b & (bins - 1)] = 0;
+        for (uint32_t b = tid; b < 16 * bins; b += 1024) cnt[b >> a.bits][b & (bins - 1)] = 0;
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < kBucketRounds; ++r)
-            if (r < rounds) {
-                const bool on = base + r * 64 < m;
-                const uint32_t d = (k[r] >> sh) & (bins - 1);
-                const uint64_t same = match<kBucketBits>(d, on, bits);
-                const int first = __ffsll((unsigned long long)same) - 1;
-                uint32_t old = 0;
-                if (on && lane == first) old = atomicAdd(&cnt[w][d], (uint32_t)__popcll(same));
-                place[r] = __shfl(old, first) + __popcll(same & below(lane));
-            }
+            if (r < rounds)
+                place[r] = take_places(cnt[w], (k[r] >> sh) & (bins - 1), base + r * 64 < m, a.bits, lane);
         __syncthreads();
-        // where each wave's entries of a digit go: after all smaller digits and the earlier waves'
-        uint32_t c[16], sum = 0;
-        if ((uint32_t)tid < bins) {
-#pragma unroll
-            for (int q = 0; q < 16; ++q) c[q] = cnt[q][tid];
-#pragma unroll
-            for (int q = 0; q < 16; ++q) sum += c[q];
-        }
-        const uint32_t inc = wave_scan(sum, lane);
-        if (lane == 63) wsum[0][w] = inc;
-        __syncthreads();
-        uint32_t to = inc - sum;
-        for (int q = 0; q < w; ++q) to += wsum[0][q];
-        if ((uint32_t)tid < bins) {
-#pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                cnt[q][tid] = to;
-                to += c[q];
-            }
-        }
-        __syncthreads();
+        digit_places(cnt, wsum[0], bins);
 #pragma unroll
         for (int r = 0; r < kBucketRounds; ++r)
             if (r < rounds && base + r * 64 < m) {
-                const uint32_t d = cnt[w][(k[r] >> sh) & (bins - 1)] + place[r];
-                if (pass == passes - 1)
-                    out[d] = make_uint2(k[r], p[r]);
+                const uint32_t to = cnt[w][(k[r] >> sh) & (bins - 1)] + place[r];
+                if (pass == a.passes - 1)
+                    out[to] = make_uint2(k[r], p[r]);
                 else
-                    pos[d] = p[r];
+                    pos[to] = p[r];
             }
         __syncthreads();
     }
@@ -481,25 +565,30 @@ __device__ __forceinline__ void sum_subgroups(Vec<float, VEC>* part, float* acc,
 // ---- few entries: one launch, a workgroup per entry.  The first of the entries that name a row
 // sums them all (each subgroup every NS-th of them, joined through LDS); other workgroups store the
 // zeros of the rows that no id names.
-constexpr int kFewMost = 256;
+constexpr int kFewMost = 1024;
 constexpr int kFewRows = 1024;  // rows per zeroing workgroup, at most
 
 template <typename GT, typename OT, typename I, int VEC>
 __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
+    constexpr int PER = kFewMost / 256;
     __shared__ Vec<float, VEC> part[256];
-    __shared__ uint32_t match[kFewMost];
-    __shared__ uint32_t count[4], first[4];
+    __shared__ uint16_t match[kFewMost];
+    __shared__ uint32_t count[PER][4];
     __shared__ uint8_t named[kFewRows];
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const int L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
     const int64_t col = ((int64_t)blockIdx.y * L + ln) * VEC;
     const bool on = col < a.D;
-    const uint32_t mine = (uint32_t)tid < a.n ? a.ids.get(tid, a.V) : a.V;
+    uint32_t mine[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) mine[k] = k * 256 + tid < (int)a.n ? a.ids.get(k * 256 + tid, a.V) : a.V;
     if (blockIdx.x >= a.n) {
         const uint32_t r0 = (blockIdx.x - a.n) * a.rows;
         for (uint32_t k = tid; k < a.rows; k += 256) named[k] = 0;
         __syncthreads();
-        if (mine < a.V && mine >= r0 && mine - r0 < a.rows) named[mine - r0] = 1;
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (mine[k] < a.V && mine[k] >= r0 && mine[k] - r0 < a.rows) named[mine[k] - r0] = 1;
         __syncthreads();
         const float z[VEC] = {};
         for (uint32_t k = s; k < a.rows && r0 + k < a.V; k += NS)
@@ -508,20 +597,23 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
     }
     const uint32_t v = a.ids.get(blockIdx.x, a.V);
     if (v >= a.V) return;
-    const uint64_t same = __ballot(mine == v);
-    if (lane == 0) {
-        count[w] = __popcll(same);
-        first[w] = same ? w * 64 + __ffsll((unsigned long long)same) - 1 : ~0u;
-    }
-    __syncthreads();
-    if (min(min(first[0], first[1]), min(first[2], first[3])) < blockIdx.x) return;
-    uint32_t at = 0, m = 0;
+    uint64_t same[PER];
+    int earlier = 0;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        if (q < w) at += count[q];
-        m += count[q];
+    for (int k = 0; k < PER; ++k) {
+        same[k] = __ballot(mine[k] == v);
+        earlier |= mine[k] == v && k * 256 + tid < (int)blockIdx.x;
+        if (lane == 0) count[k][w] = __popcll(same[k]);
     }
-    if (mine == v) match[at + __popcll(same & ((1ull << lane) - 1))] = tid;
+    if (__syncthreads_or(earlier)) return;
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (q == w && mine[k] == v) match[m + __popcll(same[k] & below(lane))] = (uint16_t)(k * 256 + tid);
+            m += count[k][q];
+        }
     __syncthreads();
     float acc[VEC] = {};
     if (on) {
@@ -542,7 +634,8 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
 
 // ---- few rows: no sort.  Every subgroup keeps a table of sums in LDS, its own, so a workgroup's
 // entries are read once and in order; the subgroups' and then the workgroups' tables are added.
-constexpr int kTableMost = 64;  // V * VEC: 64 KB of LDS, two workgroups per compute unit
+// 500k ids of rows of 32 floats: 16 rows 20.8 us (sorted: 37.8), 32 rows 28.6 (sorted: 37.6).
+constexpr int kTableMost = 128;  // V * VEC: 128 KB of LDS
 
 template <typename GT, typename I, int VEC>
 __global__ __launch_bounds__(256) void embed_table_kernel(const SumArgs<I> a) {
@@ -841,7 +934,7 @@ static BwdPlan bwd_plan(int64_t V, int64_t n, int64_t D, int vec) {
     };
     p.form = n <= kFewMost ? kFew : V * vec <= kTableMost ? kTable : n <= kBucketMost ? kBucket : kRadix;
     if (p.form == kTable) {
-        int64_t blocks = 512 / p.slabs;  // two per compute unit
+        int64_t blocks = (V * vec > 64 ? 256 : 512) / p.slabs;  // as many as the tables leave room for
         if (blocks < 1) blocks = 1;
         const int64_t step = 8 * NS, rows = (n + blocks - 1) / blocks;
         p.rows = (uint32_t)((rows + step - 1) / step * step);
@@ -852,6 +945,7 @@ static BwdPlan bwd_plan(int64_t V, int64_t n, int64_t D, int vec) {
         p.run = (n / (NS * kSumRun) + 1) * p.slabs < 256 ? 8 : kSumRun;
         p.blocks = (uint32_t)((n + NS * p.run - 1) / (NS * p.run));
         p.list_a = take((size_t)n * 8);
+        if (n > kBucketKeep) p.list_b = take((size_t)n * 8);
         p.head = take((size_t)p.blocks * D * 4);
         p.tail = take((size_t)p.blocks * D * 4);
         int key_bits = 1;
@@ -866,7 +960,6 @@ static BwdPlan bwd_plan(int64_t V, int64_t n, int64_t D, int vec) {
         p.bits = p.passes ? (key_bits + p.passes - 1) / p.passes : 0;
         if (p.form == kRadix) {
             p.tiles = (uint32_t)((n + kSortTile - 1) / kSortTile);
-            p.list_b = take((size_t)n * 8);
             p.hist = take(((size_t)p.tiles << p.bits) * 4);
             p.total = take((4ull << p.bits));
             p.ascend = take(((size_t)p.tiles + 1) * 4);
@@ -911,8 +1004,8 @@ static void launch_sort(const BwdPlan& p, char* w, SumArgs<I>& a, const ZeroPart
     uint32_t zb, zb1;
     if (p.form == kBucket) {
         const ZeroPart all = take_zeros(z, 0, 1, zb);
-        hipLaunchKernelGGL((sort_bucket_kernel<I>), dim3(p.buckets + zb), dim3(1024), 0, s, a.n, a.ids, a.V, p.shift,
-                           p.passes, p.bits, la, p.buckets, all);
+        const BucketArgs<I> t{a.n, a.V, a.ids, p.shift, p.passes, p.bits, p.buckets, la, lb};
+        hipLaunchKernelGGL((sort_bucket_kernel<I>), dim3(p.buckets + zb), dim3(1024), 0, s, t, all);
         a.list = la;
         return;
     }

@@ -155,7 +155,6 @@ def embedding(weight, ids, scale=1.0, dtype=None):
     return _lookup(weight, flat, ids.shape, float(scale), dtype, index)
 
 
-@torch.no_grad()
 def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
     """The lookup's gradient by itself: dw[v] = scale * sum of grad's rows whose id is v.
 

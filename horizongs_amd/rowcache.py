@@ -73,7 +73,6 @@ def _check_slots(slots, n):
     check_ids(slots)
 
 
-@torch.no_grad()
 def rowcache_write(cache, rows, slots=None):
     """Quantise rows [n, dim] (float32, float16 or bfloat16, contiguous columns) into their slots (int32 /
     int64 [n]; None: slots 0 .. n - 1).  A row whose slot lies outside the cache (-1 by custom) is left
@@ -101,7 +100,6 @@ def rowcache_write(cache, rows, slots=None):
               *_slot_args(slots), codes.data_ptr(), cs, scales.data_ptr(), ss, ws.data_ptr() if ws_b else None, ws_b)
 
 
-@torch.no_grad()
 def rowcache_read(cache, slots=None, dtype=torch.float32):
     """Rows [n, dim] of the named slots (int32 / int64 [n]; None: every slot) in `dtype`: code * scale in
     f32, rounded once.  A slot outside the cache reads zeros."""

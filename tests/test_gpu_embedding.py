@@ -126,7 +126,10 @@ def test_grad(V, n, D, gt, ot):
     (300, 256, 2048, "one"), (300, 257, 2048, "one"), (1_000_000, 250_000, 32, "sorted"), (4096, 65_536, 5, "mixed"),
     (2048, 100_000, 33, "reversed"), (70_000, 40_000, 8, "one"), (2048, 100_000, 33, "sorted"),
     (50_000, 30_000, 24, "tail"), (3000, 20_000, 8, "none"), (1_500_000, 17_000, 4, "tail"), (600, 9000, 48, "tail"),
-    (600, 16_384, 8, "one"), (1 << 20, 16_000, 8, "mixed"), (200, 5000, 100, "uniform")])
+    (600, 16_384, 8, "one"), (1 << 20, 16_000, 8, "mixed"), (200, 5000, 100, "uniform"),
+    (90, 32_768, 12, "uniform"), (90, 32_769, 12, "uniform"), (1 << 20, 30_000, 8, "mixed"), (1 << 20, 60_000, 8, "mixed"), (1 << 20, 8193, 8, "one"),
+    (300, 8192, 24, "mixed"), (300, 8193, 24, "mixed"), (300, 1024, 2048, "one"), (300, 1025, 2048, "one"),
+    (200_000_000, 30_000, 1, "mixed")])
 def test_grad_of_whole_numbers_is_exact(V, n, D, kind):
     ids = make_ids(kind, V, n, n).to(DEV)
     g = torch.randint(-8, 9, (n, D), generator=gen(V)).to(DEV)

@@ -87,7 +87,7 @@ def test_c_entries_refuse_before_any_launch():
     refused(lib.hgsr_embed_bwd(4, 1, 4, f, 0, 4, f, 0, 1, 1.0, t, 0, 3, 0, f, 1 << 20, None), "stride")
     refused(lib.hgsr_embed_bwd(4, 1, 4, f, 0, 4, f, 0, 1, 1.0, None, 0, 4, 0, f, 1 << 20, None), "null")
     refused(lib.hgsr_embed_bwd(4, 1, 4, f, 0, 4, f, 0, 1, 1.0, t, 0, 5, 0, f, 1 << 20, None), "contiguous")
-    for V, n in ((4, 1000), (1000, 1000), (1000, 100_000)):  # each form that keeps a workspace
+    for V, n in ((4, 2000), (1000, 2000), (1000, 100_000)):  # each form that keeps a workspace
         need = lib.hgsr_embed_bwd_ws_bytes(V, n, 4)
         refused(lib.hgsr_embed_bwd(V, n, 4, f, 0, 4, f, 0, 1, 1.0, t, 0, 4, 0, f, 0, None), "workspace", -3)
         refused(lib.hgsr_embed_bwd(V, n, 4, f, 0, 4, f, 0, 1, 1.0, t, 0, 4, 0, None, need, None), "workspace", -3)
