@@ -25,12 +25,12 @@ namespace hgsr {
 // ------------------------------------------------------------------------------------- lookup
 
 template <typename WT, typename OT, typename I, int VEC, bool STREAM>
-__global__ __launch_bounds__(256) void embed_fwd_kernel(uint32_t chunks, FastDiv per_row, uint32_t V,
+__global__ __launch_bounds__(256) void embed_fwd_kernel(uint32_t chunks, FastDiv per_row, uint32_t V, uint32_t D,
                                                         const WT* __restrict__ w, int64_t wstride, RowIds<I> ids,
                                                         int64_t row0, float scale, OT* __restrict__ out) {
     const uint32_t c = blockIdx.x * 256 + threadIdx.x;
     if (c >= chunks) return;
-    const uint32_t r = per_row.div(c), col = (c - r * per_row.d) * VEC;
+    const uint32_t r = per_row.div(c), col = min((c - r * per_row.d) * VEC, D - VEC);  // rows end on a whole piece
     const uint32_t id = ids.get(row0 + r, V);
     Vec<OT, VEC> o;
     if (id < V) {
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(uint32_t chunks, FastDiv
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o.v[k] = (OT)0.0f;
     }
-    OT* to = out + (row0 + r) * ((int64_t)per_row.d * VEC) + col;
+    OT* to = out + (row0 + r) * (int64_t)D + col;
     if (STREAM)
         stream_vec<OT, VEC>(to, o);
     else
@@ -528,10 +528,32 @@ struct SumArgs {
     uint8_t* named;      // table form: [blocks][V]
 };
 
+// The columns of a lane.  A row whose length no VEC divides ends on a whole piece all the same: its last
+// lane's columns start before the piece (`skip` of them are the previous lane's too, and get the same
+// values from both, except where something is added to them).
+template <int VEC>
+struct Cols {
+    int64_t col;
+    int skip;
+    bool on;
+    __device__ __forceinline__ Cols(int64_t D, int lanes, int ln) {
+        const int64_t c = ((int64_t)blockIdx.y * lanes + ln) * VEC;
+        on = c < D;
+        col = c < D - VEC ? c : D - VEC;
+        skip = on ? (int)(c - col) : 0;
+    }
+};
+
 template <typename OT, int VEC, bool STREAM = false, typename I>
-__device__ __forceinline__ void put_row(const SumArgs<I>& a, uint32_t v, int64_t col, const float* acc) {
-    OT* p = static_cast<OT*>(a.dw) + (int64_t)v * a.dwstride + col;
+__device__ __forceinline__ void put_row(const SumArgs<I>& a, uint32_t v, const Cols<VEC>& c, const float* acc) {
+    OT* p = static_cast<OT*>(a.dw) + (int64_t)v * a.dwstride + c.col;
     Vec<OT, VEC> o;
+    if (a.accumulate && c.skip) {
+#pragma unroll
+        for (int k = 1; k < VEC; ++k)
+            if (k >= c.skip) p[k] = (OT)((float)p[k] + acc[k] * a.scale);
+        return;
+    }
     if (a.accumulate) {
         o = load_vec<OT, VEC>(p);
 #pragma unroll
@@ -584,8 +606,9 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
     __shared__ uint8_t named[kFewRows];
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const int L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
-    const int64_t col = ((int64_t)blockIdx.y * L + ln) * VEC;
-    const bool on = col < a.D;
+    const Cols<VEC> c(a.D, L, ln);
+    const int64_t col = c.col;
+    const bool on = c.on;
     uint32_t mine[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) mine[k] = k * 256 + tid < (int)a.n ? a.ids.get(k * 256 + tid, a.V) : a.V;
@@ -599,7 +622,7 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
         __syncthreads();
         const float z[VEC] = {};
         for (uint32_t k = s; k < a.rows && r0 + k < a.V; k += NS)
-            if (on && !named[k]) put_row<OT, VEC>(a, r0 + k, col, z);
+            if (on && !named[k]) put_row<OT, VEC>(a, r0 + k, c, z);
         return;
     }
     const uint32_t v = a.ids.get(blockIdx.x, a.V);
@@ -636,7 +659,7 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
         }
     }
     sum_subgroups<VEC>(part, acc, L, m < (uint32_t)NS ? (int)m : NS);
-    if (s == 0 && on) put_row<OT, VEC>(a, v, col, acc);
+    if (s == 0 && on) put_row<OT, VEC>(a, v, c, acc);
 }
 
 // ---- few rows: no sort.  Every subgroup keeps a table of sums in LDS, its own, so a workgroup's
@@ -650,15 +673,16 @@ __global__ __launch_bounds__(256) void embed_table_kernel(const SumArgs<I> a) {
     Vec<float, VEC>* tab = reinterpret_cast<Vec<float, VEC>*>(smem);  // [V][256]
     __shared__ uint8_t named[kTableMost];
     const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
-    const int64_t col = ((int64_t)blockIdx.y * L + ln) * VEC;
-    const bool on = col < a.D;
+    const Cols<VEC> c(a.D, L, ln);
+    const int64_t col = c.col;
+    const bool on = c.on;
     Vec<float, VEC> zero;
 #pragma unroll
     for (int c = 0; c < VEC; ++c) zero.v[c] = 0.0f;
     for (uint32_t v = 0; v < a.V; ++v) tab[v * 256 + tid] = zero;
     if (tid < kTableMost) named[tid] = 0;
     __syncthreads();
-    const GT* g = static_cast<const GT*>(a.g) + (on ? col : 0);
+    const GT* g = static_cast<const GT*>(a.g) + col;
     const uint64_t i1 = min((uint64_t)a.n, ((uint64_t)blockIdx.x + 1) * a.rows);
     for (uint64_t i0 = (uint64_t)blockIdx.x * a.rows + s; i0 < i1; i0 += 8 * NS) {
         uint32_t id[8];
@@ -698,8 +722,9 @@ __global__ __launch_bounds__(1024) void embed_table_join_kernel(const SumArgs<I>
     __shared__ Vec<float, VEC> part[1024];
     const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 1024 / L;
     const uint32_t v = blockIdx.x, share = (a.blocks + NS - 1) / NS;
-    const int64_t col = ((int64_t)blockIdx.y * L + ln) * VEC;
-    const bool on = col < a.D;
+    const Cols<VEC> c(a.D, L, ln);
+    const int64_t col = c.col;
+    const bool on = c.on;
     float acc[VEC] = {};
     int hit = 0;
     const uint32_t b1 = min(a.blocks, (s + 1) * share);
@@ -714,7 +739,7 @@ __global__ __launch_bounds__(1024) void embed_table_join_kernel(const SumArgs<I>
     }
     hit = __syncthreads_or(hit);
     sum_subgroups<VEC>(part, acc, L, NS);
-    if (s == 0 && on && (hit || !a.accumulate)) put_row<OT, VEC>(a, v, col, acc);
+    if (s == 0 && on && (hit || !a.accumulate)) put_row<OT, VEC>(a, v, c, acc);
 }
 
 // ---- the general form: every subgroup walks `run` consecutive entries of the sorted list, and a
@@ -736,8 +761,9 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs<I> a) {
     const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
     const uint32_t E = NS * a.run, block = xcd_remap(blockIdx.x, gridDim.x);
     uint32_t* pos = key + E + 2;
-    const int64_t col = ((int64_t)blockIdx.y * L + ln) * VEC;
-    const bool on = col < a.D, asc = a.ascend && *a.ascend;
+    const Cols<VEC> c(a.D, L, ln);
+    const int64_t col = c.col;
+    const bool on = c.on, asc = a.ascend && *a.ascend;
     constexpr uint32_t NONE = ~0u;
     const uint32_t i0 = block * E;
 #pragma unroll
@@ -752,7 +778,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs<I> a) {
     if (tid == 0) key[0] = i0 ? sorted_id(a, asc, i0 - 1) : NONE;
     if (tid == 64) key[1 + E] = i0 + E < a.n ? sorted_id(a, asc, i0 + E) : NONE;
     __syncthreads();
-    const GT* g = static_cast<const GT*>(a.g) + (on ? col : 0);
+    const GT* g = static_cast<const GT*>(a.g) + col;
     const int e0 = s * a.run;
     float acc[VEC] = {};
     bool head = key[e0] == key[1 + e0];  // the first run began before this subgroup
@@ -778,7 +804,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs<I> a) {
                 part[head ? 0 : 1][tid] = o;
                 st |= head ? (goes_on ? 3 : 1) : 4;
             } else if (on) {
-                put_row<OT, VEC, true>(a, v, col, acc);
+                put_row<OT, VEC, true>(a, v, c, acc);
             }
             head = false;
 #pragma unroll
@@ -804,7 +830,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs<I> a) {
         if (open)
             keep(a.tail);
         else
-            put_row<OT, VEC, true>(a, key[e0 + a.run], col, acc);
+            put_row<OT, VEC, true>(a, key[e0 + a.run], c, acc);
     }
     if (s == 0 && (st & 1)) {  // the run that an earlier workgroup began
 #pragma unroll
@@ -859,10 +885,10 @@ __device__ __forceinline__ void zero_between(const SumArgs<I>& a, uint32_t r0) {
         }
     }
     __syncthreads();
-    const int64_t col = ((int64_t)blockIdx.y * L + ln) * VEC;
+    const Cols<VEC> c(a.D, L, ln);
     const float z[VEC] = {};
     for (uint32_t k = s; k < a.rows && r0 + k < a.V; k += NS)
-        if (col < a.D && !named[k]) put_row<OT, VEC, true>(a, r0 + k, col, z);
+        if (c.on && !named[k]) put_row<OT, VEC, true>(a, r0 + k, c, z);
 }
 
 // One workgroup per workgroup of the sums: if a run begins in it and goes on, its tail and the
@@ -894,8 +920,9 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const SumArgs<I> a) {
     }
     __syncthreads();
     const uint32_t m = s_last - b, share = (m + NS - 1) / NS;
-    const int64_t col = ((int64_t)blockIdx.y * L + ln) * VEC;
-    const bool on = col < a.D;
+    const Cols<VEC> c(a.D, L, ln);
+    const int64_t col = c.col;
+    const bool on = c.on;
     float acc[VEC] = {};
     if (on) {
         const uint32_t j0 = b + 1 + min(m, s * share), j1 = b + 1 + min(m, (s + 1) * share);
@@ -912,7 +939,7 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const SumArgs<I> a) {
         for (int c = 0; c < VEC; ++c) acc[c] += p[c];
     }
     sum_subgroups<VEC>(part, acc, L, m < (uint32_t)NS ? (int)m : NS);
-    if (s == 0 && on) put_row<OT, VEC>(a, v, col, acc);
+    if (s == 0 && on) put_row<OT, VEC>(a, v, c, acc);
 }
 
 // ---------------------------------------------------------------------------------- launches
@@ -1122,13 +1149,13 @@ struct FwdArgs {
 
 template <typename WT, typename OT, typename I, int VEC, bool STREAM>
 static void launch_fwd(const FwdArgs& a, hipStream_t s) {
-    const uint32_t per_row = (uint32_t)(a.D / VEC);
+    const uint32_t per_row = (uint32_t)((a.D + VEC - 1) / VEC);
     const RowIds<I> ids{static_cast<const I*>(a.ids), a.ids_stride};
     const int64_t most = ((int64_t)1 << 30) / per_row;  // rows per launch: at most 2^30 pieces
     for (int64_t r0 = 0; r0 < a.n; r0 += most) {
         const uint32_t chunks = (uint32_t)((a.n - r0 < most ? a.n - r0 : most) * per_row);
         hipLaunchKernelGGL((embed_fwd_kernel<WT, OT, I, VEC, STREAM>), dim3((chunks + 255) / 256), dim3(256), 0, s, chunks,
-                           fast_div(per_row), (uint32_t)a.V, static_cast<const WT*>(a.w),
+                           fast_div(per_row), (uint32_t)a.V, (uint32_t)a.D, static_cast<const WT*>(a.w),
                            a.wstride, ids, r0, a.scale, static_cast<OT*>(a.out));
     }
 }
@@ -1181,9 +1208,7 @@ extern "C" int hgsr_embed_fwd(int64_t V, int64_t n, int64_t D, const void* weigh
     if (n == 0) return HGSR_OK;
     HGSR_REQUIRE(ids && out && (weight || V == 0), "embed_fwd: null pointer");
     const int most = wtype != HGSR_F32 && otype != HGSR_F32 ? 8 : 4;
-    int vec = vec_width(most, D, wstride, weight, elem_size(wtype));
-    const int vo = vec_width(most, D, D, out, elem_size(otype));
-    if (vo < vec) vec = vo;
+    const int vec = vec_width(most, D);
     const FwdArgs a{V, n, D, wstride, ids_stride, weight, ids, ids64, scale, out};
     hipStream_t s = as_stream(stream);
     {
@@ -1201,8 +1226,8 @@ extern "C" int hgsr_embed_fwd(int64_t V, int64_t n, int64_t D, const void* weigh
 extern "C" size_t hgsr_embed_bwd_ws_bytes(int64_t V, int64_t n, int64_t D) {
     if (V <= 0 || n <= 0 || D < 1) return 0;
     size_t most = 0;
-    for (int vec = 1; vec <= 8; vec <<= 1) {  // the call picks the width by the tensors' alignment
-        const size_t b = bwd_plan(V, n, D, vec).bytes;
+    for (int widest = 4; widest <= 8; widest <<= 1) {  // of a 32-bit and of a 16-bit gradient
+        const size_t b = bwd_plan(V, n, D, vec_width(widest, D)).bytes;
         if (b > most) most = b;
     }
     return most;
@@ -1230,9 +1255,7 @@ extern "C" int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, in
     }
     HGSR_REQUIRE(g && ids, "embed_bwd: null pointer");
     const int most = gtype == HGSR_F32 ? 4 : 8;
-    int vec = vec_width(most, D, gstride, g, elem_size(gtype));
-    const int vo = vec_width(most, D, dwstride, dw, elem_size(dwtype));
-    if (vo < vec) vec = vo;
+    const int vec = vec_width(most, D);
     const BwdPlan p = bwd_plan(V, n, D, vec);
     if (p.bytes > ws_bytes || (p.bytes && !ws)) {
         set_error("embed_bwd: workspace of %zu bytes, %zu needed", ws ? ws_bytes : (size_t)0, p.bytes);

@@ -4,10 +4,11 @@
 //   write  s = max(max |x| over a group of columns * (1 / top), 2^-100),  code = round(x / s)
 //   read   x' = code * s
 //
-// Both are bound by memory: a lane moves 8 consecutive columns of a row (4 of an f32 row that is
-// read), the lanes of a group find its maximum among themselves.  500k rows of 32 floats, every other
-// slot of a million: the write 24.7 us in its three launches (84 MB, 3.4 TB/s; the slots' lines are
-// stored in part), the read 16.0 (5.2 TB/s); 16k rows of 2048 read to bf16: 16.4 us (6.0 TB/s).
+// Both are bound by memory: a write's lane moves 16 consecutive columns of a row, a read's what fills
+// 16 bytes of its output; the lanes of a group find its maximum among themselves.  500k rows of 32
+// floats, every other slot of a million: the write 24.5 us in its three launches (84 MB, 3.4 TB/s; the
+// slots' lines are stored in part), the read 16.2 (5.2 TB/s); 16k rows of 2048 read to bf16: 16.4 us
+// (6.0 TB/s).
 #include "rows.h"
 
 namespace hgsr {
@@ -16,9 +17,10 @@ constexpr float kScaleFloor = 0x1p-100f;
 
 template <typename I>
 struct CacheArgs {
-    uint32_t capacity, chunks, width;  // chunks: lanes' pieces of this launch; width: pieces per row
+    uint32_t capacity, chunks;         // chunks: lanes' pieces of this launch
     FastDiv per_row;
-    int64_t row0, n, D;
+    int64_t row0, n;
+    uint32_t D;
     int group, glog;                   // group = 1 << glog columns
     uint8_t* codes;
     float* scales;
@@ -36,17 +38,6 @@ __device__ __forceinline__ uint32_t slot_of(const CacheArgs<I>& a, int64_t i) {
     return a.slots.get(i, a.capacity);
 }
 
-// The rounding of x / s is that of the exact quotient.  x * (1 / s) is off by at most 2^-23 of it, so its
-// rounding is the quotient's unless it lies that near to the border of two codes (5 of 100,000 int8
-// values, 1 of 100,000 e4m3 ones); a wave that holds such a value divides exactly.  (500k rows of 32
-// floats: 19.5 us, 20.2 with every quotient exact.)
-template <int FMT>
-__device__ __forceinline__ bool near_border(float q, float x) {
-    if (FMT == HGSR_INT8) return fabsf(q - rintf(q)) > 0.5f - 0x1p-15f;  // |q| <= 127: off by at most 2^-16
-    const uint32_t below = __float_as_uint(q) & 0xfffffu;  // the mantissa's bits behind the code's three
-    return below - 0x7fffcu <= 8u || (fabsf(q) < 0x1p-6f && x != 0.0f);  // subnormal codes: fewer than three
-}
-
 // x / s as a float whose last bit stands for what lies below it ("round to odd"): any later
 // rounding to fewer bits gives what rounding the exact quotient would.  inv = 1 / s, s a normal
 // float; q is within one step of the quotient after its correction, and the remainder x - q s of
@@ -61,13 +52,56 @@ __device__ __forceinline__ float quotient_odd(float x, float s, float inv) {
     return q;
 }
 
-template <int FMT>
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
-    if (FMT == HGSR_INT8)
-        return ((uint32_t)(int)rintf(a) & 255u) | ((uint32_t)(int)rintf(b) & 255u) << 8 |
-               ((uint32_t)(int)rintf(c) & 255u) << 16 | (uint32_t)(int)rintf(d) << 24;
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+// The codes of VEC values of a group, four to a word.  The rounding of x / s is that of the exact
+// quotient: q = x * (1 / s) is off by at most 2^-23 of it, so its rounding is the quotient's unless q lies
+// that near to the border of two codes (5 of 100,000 int8 values, 1 of 100,000 e4m3 ones); a wave that
+// holds such a value divides exactly.  16-bit rows are bound by this arithmetic: 16k x 2048 bf16 take
+// 37 us with a comparison for every value and separate conversions.
+template <int FMT, int VEC>
+__device__ __forceinline__ void encode(const float* x, float s, float inv, uint32_t* w) {
+#pragma clang fp contract(off)
+    if (FMT == HGSR_INT8) {
+        // q + 1.5 2^23 rounds q to a whole number and holds it in its low bits; |q| <= 127: q is off by
+        // at most 2^-16
+        constexpr float kWhole = 12582912.0f;
+        uint32_t t[VEC];
+        float off = 0.0f;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            const float q = x[k] * inv, r = q + kWhole;
+            off = fmaxf(off, fabsf(q - (r - kWhole)));
+            t[k] = __float_as_uint(r);
+        }
+        if (__any(off > 0.5f - 0x1p-15f)) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) t[k] = __float_as_uint(rintf(quotient_odd(x[k], s, inv)) + kWhole);
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; k += 4)
+            w[k / 4] = __builtin_amdgcn_perm(t[k + 1], t[k], 0x0c0c0400u) |
+                       __builtin_amdgcn_perm(t[k + 3], t[k + 2], 0x04000c0cu);
+        return;
+    }
+    // near: how far the mantissa's 20 bits behind the code's three are from the border, 0x80000; low: the
+    // smallest magnitude but 0 (below 2^-6 codes have fewer bits)
+    float y[VEC];
+    uint32_t near = ~0u, low = ~0u;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+        y[k] = x[k] * inv;
+        const uint32_t b = __float_as_uint(y[k]);
+        near = min(near, (b - 0x7fffcu) & 0xfffffu);
+        low = min(low, (b & 0x7fffffffu) - 1u);
+    }
+    if (__any(near <= 8u || low < 0x3c800000u - 1u)) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) y[k] = quotient_odd(x[k], s, inv);
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4) {
+        const int v = __builtin_amdgcn_cvt_pk_fp8_f32(y[k], y[k + 1], 0, false);
+        w[k / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[k + 2], y[k + 3], v, true);
+    }
 }
 template <int FMT>
 __device__ __forceinline__ void decode4(uint32_t w, float* o) {
@@ -133,38 +167,39 @@ __global__ __launch_bounds__(256) void slot_last_kernel(uint32_t n, RowIds<I> sl
     }
 }
 
-// VEC consecutive columns per lane; ALIGNED: whole pieces, moved as vectors.  FEW: no more than
+// VEC consecutive columns per lane, fewer where the row ends.  FEW: no more than
 // kFewSlots rows, whose repeated slots are found here, by a group's lanes among the later rows.
 constexpr int kFewSlots = 1024;
 
-template <typename XT, typename I, int FMT, int VEC, bool ALIGNED, bool FEW>
+template <typename XT, typename I, int FMT, int VEC, bool FEW>
 __global__ __launch_bounds__(256) void rowcache_write_kernel(const CacheArgs<I> a) {
     __shared__ uint32_t slots[FEW ? kFewSlots : 1];
-    // an XCD's workgroups take consecutive rows: slots in order then share its L2's lines
-    const uint32_t c = xcd_remap(blockIdx.x, gridDim.x) * 256 + threadIdx.x;
+    // Narrow rows: an XCD's workgroups take consecutive ones, so that slots in order share its L2's lines
+    // (500k rows of 32 floats 24.5 us, 25.3 without).  Wide ones share none (16k of 2048: 41.8, 43.1 with).
+    const uint32_t c = (a.D < 128 ? xcd_remap(blockIdx.x, gridDim.x) : blockIdx.x) * 256 + threadIdx.x;
     const bool in = c < a.chunks;
     const uint32_t r = a.per_row.div(in ? c : 0);
-    const int64_t row = a.row0 + r, col = in ? (int64_t)(c - r * a.per_row.d) * VEC : a.D;
+    const int64_t row = a.row0 + r;
+    const uint32_t D = a.D, col = in ? (c - r * a.per_row.d) * VEC : D;
     const uint32_t slot = slot_of(a, row);
     float x[VEC];
     const XT* p = static_cast<const XT*>(a.x) + row * a.xstride + col;
-    if (ALIGNED) {
-        Vec<XT, VEC> v{};
-        if (col < a.D) v = load_vec<XT, VEC>(p);
+    if (col + VEC <= D) {
+        const Vec<XT, VEC> v = load_vec<XT, VEC>(p);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) x[k] = (float)v.v[k];
     } else {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) x[k] = col + k < a.D ? (float)p[k] : 0.0f;
+        for (int k = 0; k < VEC; ++k) x[k] = col + k < D ? (float)p[k] : 0.0f;
     }
     if (FEW) {
         for (uint32_t i = threadIdx.x; i < (uint32_t)a.n; i += 256) slots[i] = slot_of(a, i);
         __syncthreads();
     }
-    bool on = col < a.D && slot < a.capacity;
+    bool on = col < D && slot < a.capacity;
     if (!FEW && a.last && !*a.distinct && on) on = a.last[slot] == (int32_t)row;
     // the largest magnitude of the group as bits: infinities and NaN lie above every number
-    const int lanes = a.group / VEC;  // a power of two, <= 16
+    const int lanes = a.group / VEC;  // a power of two, <= 8
     uint32_t m = 0;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) m = max(m, __float_as_uint(x[k]) & 0x7fffffffu);
@@ -175,32 +210,21 @@ __global__ __launch_bounds__(256) void rowcache_write_kernel(const CacheArgs<I> 
     if (!on || (FEW && m == 0x80000000u)) return;
     const bool finite = m < 0x7f800000u;
     const float per = FMT == HGSR_INT8 ? 1.0f / 127.0f : 1.0f / 448.0f;
-    const float s = fmaxf(__uint_as_float(finite ? m : 0u) * per, kScaleFloor), inv = 1.0f / s;
-    float y[VEC];
-    bool near = false;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-        if (!finite) x[k] = 0.0f;
-        y[k] = x[k] * inv;
-        near |= near_border<FMT>(y[k], x[k]);
-    }
-    if (__any(near)) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) y[k] = quotient_odd(x[k], s, inv);
-    }
+    const float s = fmaxf(__uint_as_float(m) * per, kScaleFloor), inv = 1.0f / s;
     uint32_t w[VEC / 4];
+    encode<FMT, VEC>(x, s, inv, w);
 #pragma unroll
-    for (int k = 0; k < VEC; k += 4) w[k / 4] = encode4<FMT>(y[k], y[k + 1], y[k + 2], y[k + 3]);
+    for (int k = 0; k < VEC / 4; ++k) w[k] = finite ? w[k] : 0u;
     uint8_t* to = a.codes + (int64_t)slot * a.cstride + col;
-    if (ALIGNED) {
-        Vec<uint32_t, VEC / 4> o;
+    if (col + VEC <= D) {
+        Vec<uint8_t, VEC> o;
 #pragma unroll
-        for (int k = 0; k < VEC / 4; ++k) o.v[k] = w[k];
-        store_vec<uint32_t, VEC / 4>(reinterpret_cast<uint32_t*>(to), o);
+        for (int k = 0; k < VEC / 4; ++k) __builtin_memcpy(o.v + 4 * k, w + k, 4);
+        store_vec<uint8_t, VEC>(to, o);
     } else {
 #pragma unroll
         for (int k = 0; k < VEC; ++k)
-            if (col + k < a.D) to[k] = (uint8_t)(w[k / 4] >> (8 * (k & 3)));
+            if (col + k < D) to[k] = (uint8_t)(w[k / 4] >> (8 * (k & 3)));
     }
     if ((col & (a.group - 1)) == 0)
         a.scales[(int64_t)slot * a.sstride + (col >> a.glog)] = finite ? s : __builtin_nanf("");
@@ -208,37 +232,38 @@ __global__ __launch_bounds__(256) void rowcache_write_kernel(const CacheArgs<I> 
 
 // -------------------------------------------------------------------------------------- read
 
-// STREAM: the rows are stored past the caches
-template <typename OT, typename I, int FMT, int VEC, bool ALIGNED, bool STREAM>
+// STREAM: the rows are stored past the caches.  WHOLE: no row ends inside a lane's piece.
+template <typename OT, typename I, int FMT, int VEC, bool WHOLE, bool STREAM>
 __global__ __launch_bounds__(256) void rowcache_read_kernel(const CacheArgs<I> a) {
     const uint32_t c = blockIdx.x * 256 + threadIdx.x;
     if (c >= a.chunks) return;
     const uint32_t r = a.per_row.div(c);
-    const int64_t row = a.row0 + r, col = (int64_t)(c - r * a.per_row.d) * VEC;
+    const int64_t row = a.row0 + r;
+    const uint32_t D = a.D, col = (c - r * a.per_row.d) * VEC;
     const uint32_t slot = slot_of(a, row);
     float x[VEC] = {};
     if (slot < a.capacity) {
         const uint8_t* p = a.codes + (int64_t)slot * a.cstride + col;
         const float s = a.scales[(int64_t)slot * a.sstride + (col >> a.glog)];
         uint32_t w[VEC / 4];
-        if (ALIGNED) {
-            const Vec<uint32_t, VEC / 4> v = load_vec<uint32_t, VEC / 4>(reinterpret_cast<const uint32_t*>(p));
+        if (WHOLE || col + VEC <= D) {
+            const Vec<uint8_t, VEC> v = load_vec<uint8_t, VEC>(p);
 #pragma unroll
-            for (int k = 0; k < VEC / 4; ++k) w[k] = v.v[k];
+            for (int k = 0; k < VEC / 4; ++k) __builtin_memcpy(w + k, v.v + 4 * k, 4);
         } else {
 #pragma unroll
             for (int k = 0; k < VEC / 4; ++k) w[k] = 0;
 #pragma unroll
             for (int k = 0; k < VEC; ++k)
-                if (col + k < a.D) w[k / 4] |= (uint32_t)p[k] << (8 * (k & 3));
+                if (col + k < D) w[k / 4] |= (uint32_t)p[k] << (8 * (k & 3));
         }
 #pragma unroll
         for (int k = 0; k < VEC; k += 4) decode4<FMT>(w[k / 4], x + k);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) x[k] *= s;
     }
-    OT* to = static_cast<OT*>(a.x) + row * a.D + col;
-    if (ALIGNED) {
+    OT* to = static_cast<OT*>(a.x) + row * D + col;
+    if (WHOLE || col + VEC <= D) {
         Vec<OT, VEC> o;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o.v[k] = (OT)x[k];
@@ -249,44 +274,43 @@ __global__ __launch_bounds__(256) void rowcache_read_kernel(const CacheArgs<I> a
     } else {
 #pragma unroll
         for (int k = 0; k < VEC; ++k)
-            if (col + k < a.D) to[k] = (OT)x[k];
+            if (col + k < D) to[k] = (OT)x[k];
     }
 }
 
 // ---------------------------------------------------------------------------------- launches
 
-template <typename T, int FMT, int VEC, bool ALIGNED, typename I>
-static void launch(bool write, const CacheArgs<I>& a, hipStream_t s) {
+template <bool WRITE, typename T, int FMT, int VEC, typename I>
+static void launch(const CacheArgs<I>& a, hipStream_t s) {
     const dim3 block(256), grid((a.chunks + 255) / 256);
-    if (!write && ALIGNED && stream_out(a.n * a.D * (int64_t)sizeof(T)))
-        hipLaunchKernelGGL((rowcache_read_kernel<T, I, FMT, VEC, ALIGNED, ALIGNED>), grid, block, 0, s, a);
-    else if (!write)
-        hipLaunchKernelGGL((rowcache_read_kernel<T, I, FMT, VEC, ALIGNED, false>), grid, block, 0, s, a);
-    else if (a.slots.p && a.n > 1 && a.n <= kFewSlots)
-        hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, ALIGNED, true>), grid, block, 0, s, a);
-    else
-        hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, ALIGNED, false>), grid, block, 0, s, a);
+    if constexpr (WRITE) {
+        if (a.slots.p && a.n > 1 && a.n <= kFewSlots)
+            hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, true>), grid, block, 0, s, a);
+        else
+            hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, false>), grid, block, 0, s, a);
+    } else {
+        if (a.D % VEC)
+            hipLaunchKernelGGL((rowcache_read_kernel<T, I, FMT, VEC, false, false>), grid, block, 0, s, a);
+        else if (stream_out(a.n * (int64_t)a.D * (int64_t)sizeof(T)))
+            hipLaunchKernelGGL((rowcache_read_kernel<T, I, FMT, VEC, true, true>), grid, block, 0, s, a);
+        else
+            hipLaunchKernelGGL((rowcache_read_kernel<T, I, FMT, VEC, true, false>), grid, block, 0, s, a);
+    }
 }
 
-template <typename T, int FMT, int VEC, typename I>
-static void launch(bool write, bool aligned, const CacheArgs<I>& a, hipStream_t s) {
-    return aligned ? launch<T, FMT, VEC, true>(write, a, s) : launch<T, FMT, VEC, false>(write, a, s);
-}
-
-template <typename T, int VEC, typename I>
-static void launch(bool write, int format, CacheArgs<I> a, hipStream_t s) {
-    bool aligned = a.D % VEC == 0 && a.cstride % VEC == 0 && (uintptr_t)a.codes % VEC == 0;
-    aligned = aligned && (uintptr_t)a.x % 16 == 0 && a.xstride % VEC == 0;
+template <bool WRITE, typename T, int VEC, typename I>
+static void launch(int format, CacheArgs<I> a, hipStream_t s) {
     // a write's rows are whole groups of lanes, so that no group crosses a wave
-    const int64_t per_row = write ? (a.D + a.group - 1) / a.group * (a.group / VEC) : (a.D + VEC - 1) / VEC;
+    const int64_t pieces = ((int64_t)a.D + VEC - 1) / VEC, groups = ((int64_t)a.D + a.group - 1) / a.group;
+    const int64_t per_row = WRITE ? groups * (a.group / VEC) : pieces;
     const int64_t most = ((int64_t)1 << 30) / per_row;
     a.per_row = fast_div((uint32_t)per_row);
     for (a.row0 = 0; a.row0 < a.n; a.row0 += most) {
         a.chunks = (uint32_t)((a.n - a.row0 < most ? a.n - a.row0 : most) * per_row);
         if (format == HGSR_INT8)
-            launch<T, HGSR_INT8, VEC>(write, aligned, a, s);
+            launch<WRITE, T, HGSR_INT8, VEC>(a, s);
         else
-            launch<T, HGSR_E4M3, VEC>(write, aligned, a, s);
+            launch<WRITE, T, HGSR_E4M3, VEC>(a, s);
     }
 }
 
@@ -307,12 +331,12 @@ static SlotWork slot_work(void* ws, int64_t n) {
     return w;
 }
 
-template <typename I>
-static void launch(bool write, const CacheCall& c, hipStream_t s) {
+template <bool WRITE, typename I>
+static void launch(const CacheCall& c, hipStream_t s) {
     CacheArgs<I> a{};
     a.capacity = (uint32_t)c.capacity;
     a.n = c.n;
-    a.D = c.D;
+    a.D = (uint32_t)c.D;
     a.group = c.group;
     a.glog = c.group == 16 ? 4 : c.group == 32 ? 5 : c.group == 64 ? 6 : 7;
     a.codes = static_cast<uint8_t*>(c.codes);
@@ -322,27 +346,27 @@ static void launch(bool write, const CacheCall& c, hipStream_t s) {
     a.slots = RowIds<I>{static_cast<const I*>(c.slots), c.slots_stride};
     a.x = c.x;
     a.xstride = c.xstride;
-    if (write && c.slots && c.n > kFewSlots) {
+    if (WRITE && c.slots && c.n > kFewSlots) {
         const SlotWork w = slot_work(c.ws, c.n);
         hipLaunchKernelGGL((slot_clear_kernel<I>), dim3(w.tiles), dim3(256), 0, s, (uint32_t)c.n, a.slots, a.capacity, w);
         hipLaunchKernelGGL((slot_last_kernel<I>), dim3(w.tiles), dim3(256), 0, s, (uint32_t)c.n, a.slots, a.capacity, w);
         a.last = w.last;
         a.distinct = w.distinct;
     }
-    // f32 rows: a write moves 8 columns per lane (27.3 us for 500k rows of 32; 34.3 with 4), a read 4 (16.8
-    // us; 18.6 with 8: its 16-byte stores would be 32 bytes apart)
-    if (c.type == HGSR_F32 && write)
-        launch<float, 8>(write, c.format, a, s);
-    else if (c.type == HGSR_F32)
-        launch<float, 4>(write, c.format, a, s);
+    // Columns per lane: a write 16, the smallest group (16k rows of 2048 bf16 in any order 34 us, 38 with
+    // 8); a read what makes its stores 16 bytes (500k rows of 32 floats 16.2 us; 18.6 with 8 columns, whose
+    // two stores are 32 bytes apart).
+    if (c.type == HGSR_F32)
+        launch<WRITE, float, WRITE ? 16 : 4>(c.format, a, s);
     else if (c.type == HGSR_F16)
-        launch<f16_t, 8>(write, c.format, a, s);
+        launch<WRITE, f16_t, WRITE ? 16 : 8>(c.format, a, s);
     else
-        launch<bf16_t, 8>(write, c.format, a, s);
+        launch<WRITE, bf16_t, WRITE ? 16 : 8>(c.format, a, s);
 }
 
-static void launch(bool write, const CacheCall& c, hipStream_t s) {
-    return c.slots64 ? launch<int64_t>(write, c, s) : launch<int32_t>(write, c, s);
+template <bool WRITE>
+static void launch(const CacheCall& c, hipStream_t s) {
+    return c.slots64 ? launch<WRITE, int64_t>(c, s) : launch<WRITE, int32_t>(c, s);
 }
 
 }  // namespace hgsr
@@ -387,7 +411,7 @@ extern "C" int hgsr_rowcache_write(int64_t capacity, int64_t n, int64_t D, int g
     hipStream_t s = as_stream(stream);
     {
         KernelTimer kt("rowcache_write", s);
-        launch(true, c, s);
+        launch<true>(c, s);
     }
     return check_launch("rowcache_write");
 }
@@ -403,7 +427,7 @@ extern "C" int hgsr_rowcache_read(int64_t capacity, int64_t n, int64_t D, int gr
     hipStream_t s = as_stream(stream);
     {
         KernelTimer kt("rowcache_read", s);
-        launch(false, c, s);
+        launch<false>(c, s);
     }
     return check_launch("rowcache_read");
 }

@@ -10,32 +10,74 @@ namespace hgsr {
 typedef _Float16 f16_t;
 typedef __bf16 bf16_t;
 
-// VEC elements of T in registers, moved as one access of up to 16 bytes (two for 8 floats)
+// VEC elements of T in registers (and, 16-byte aligned, in LDS)
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC > 16 ? 16 : sizeof(T) * VEC) Vec {
     T v[VEC];
 };
 
+// Moved from and to memory as accesses of up to 16 bytes wherever the elements lie: the hardware takes
+// such accesses at any element's boundary.  So the columns that a lane holds, and with them the order
+// of a sum, never depend on a tensor's address or row stride.
+template <int BYTES>
+struct Words;
+template <>
+struct Words<16> {
+    typedef uint32_t reg __attribute__((ext_vector_type(4)));
+    typedef reg word __attribute__((aligned(1), may_alias));
+};
+template <>
+struct Words<8> {
+    typedef uint32_t reg __attribute__((ext_vector_type(2)));
+    typedef reg word __attribute__((aligned(1), may_alias));
+};
+template <>
+struct Words<4> {
+    typedef uint32_t reg;
+    typedef reg word __attribute__((aligned(1), may_alias));
+};
+template <>
+struct Words<2> {
+    typedef uint16_t reg;
+    typedef reg word __attribute__((aligned(1), may_alias));
+};
+template <typename T, int VEC>
+struct Access {  // COUNT accesses of `word`
+    static constexpr int BYTES = sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16, COUNT = sizeof(T) * VEC / BYTES;
+    typedef typename Words<BYTES>::word word;
+    typedef typename Words<BYTES>::reg reg;
+};
+
 template <typename T, int VEC>
 __device__ __forceinline__ Vec<T, VEC> load_vec(const T* p) {
-    return *reinterpret_cast<const Vec<T, VEC>*>(p);
+    typedef Access<T, VEC> A;
+    Vec<T, VEC> x;
+#pragma unroll
+    for (int k = 0; k < A::COUNT; ++k) {
+        const typename A::reg r = reinterpret_cast<const typename A::word*>(p)[k];
+        __builtin_memcpy(reinterpret_cast<char*>(&x) + k * A::BYTES, &r, A::BYTES);
+    }
+    return x;
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T, VEC>& x) {
-    *reinterpret_cast<Vec<T, VEC>*>(p) = x;
+    typedef Access<T, VEC> A;
+#pragma unroll
+    for (int k = 0; k < A::COUNT; ++k) {
+        typename A::reg r;
+        __builtin_memcpy(&r, reinterpret_cast<const char*>(&x) + k * A::BYTES, A::BYTES);
+        reinterpret_cast<typename A::word*>(p)[k] = r;
+    }
 }
-
 // the same, past the caches
 template <typename T, int VEC>
 __device__ __forceinline__ void stream_vec(T* p, const Vec<T, VEC>& x) {
-    if constexpr (sizeof(x) % 4 == 0) {
-        constexpr int W = sizeof(x) / 4 < 4 ? sizeof(x) / 4 : 4;
-        typedef uint32_t words __attribute__((ext_vector_type(W)));
+    typedef Access<T, VEC> A;
 #pragma unroll
-        for (int k = 0; k < (int)sizeof(x) / (4 * W); ++k)
-            __builtin_nontemporal_store(reinterpret_cast<const words*>(&x)[k], reinterpret_cast<words*>(p) + k);
-    } else {
-        store_vec<T, VEC>(p, x);
+    for (int k = 0; k < A::COUNT; ++k) {
+        typename A::reg r;
+        __builtin_memcpy(&r, reinterpret_cast<const char*>(&x) + k * A::BYTES, A::BYTES);
+        __builtin_nontemporal_store(r, reinterpret_cast<typename A::word*>(p) + k);
     }
 }
 // Rows of more bytes than the L2 caches hold (8 x 4 MB) are stored past them: what reads them next
@@ -73,15 +115,10 @@ inline FastDiv fast_div(uint32_t d) {
 inline int elem_size(int type) { return type == HGSR_F32 ? 4 : 2; }
 inline bool type_ok(int type) { return type == HGSR_F32 || type == HGSR_F16 || type == HGSR_BF16; }
 
-// The largest of 1, 2, 4, 8 elements (at most `most`) that divides the row length and the row
-// stride and at which rows of `size`-byte elements start on an access boundary
-inline int vec_width(int most, int64_t dim, int64_t stride, const void* base, int size) {
+// columns per lane: 8, 4, 2 or 1, at most `most` and no more than the row has
+inline int vec_width(int most, int64_t dim) {
     int v = most;
-    while (v > 1) {
-        const int bytes = v * size > 16 ? 16 : v * size;
-        if (dim % v == 0 && stride % v == 0 && (uintptr_t)base % bytes == 0) break;
-        v >>= 1;
-    }
+    while (v > dim) v >>= 1;
     return v;
 }
 

@@ -7,8 +7,9 @@
 
 Tables and rows may be float32, float16 or bfloat16; sums are f32, rounded once.  An id outside
 [0, num_rows) (-1 by custom) is padding: its row is zeros and it takes no part in the gradient --
-there is no host read that could raise.  Gradients are summed in an order that the ids alone set,
-so they are the same bits on every run.  There is no CPU path.
+there is no host read that could raise.  Gradients are summed in an order that the ids, the sizes
+and the types set, so they are the same bits on every run, wherever the tensors lie.  There is no
+CPU path.
 """
 from __future__ import annotations
 
@@ -161,7 +162,8 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
     grad [*ids.shape, D]; returns dw [num_rows, D] in `dtype` (default: grad's), zeros in rows that no
     id names.  With out [num_rows, D] (contiguous columns, rows that do not overlap) the sums are added
     to its named rows instead -- each row's sum and its old value are added in f32 and rounded once,
-    the other rows are left as they are -- and out is returned."""
+    the other rows are left as they are -- and out, which must not share memory with grad, is
+    returned."""
     type_code(grad.dtype)
     check_ids(ids)
     if grad.dim() < 1 or grad.shape[:-1] != ids.shape:

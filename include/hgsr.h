@@ -609,9 +609,10 @@ enum { HGSR_F32 = 0, HGSR_F16 = 1, HGSR_BF16 = 2 };
 int hgsr_embed_fwd(int64_t V, int64_t n, int64_t D, const void* weight, int wtype, int64_t wstride, const void* ids,
                    int ids64, int64_t ids_stride, float scale, void* out, int otype, hgsr_stream_t stream);
 /* Its gradient, dw[v, :] = scale * sum over i with ids[i] = v of g[i, :], summed in f32 in an
- * order that the ids alone set (no float atomics: the same bits on every run) and rounded once.
- * accumulate = 0: every row of dw is written, zeros where no id names it; accumulate = 1: the
- * sums are added to dw's named rows, the others are neither read nor written.  Padding ids take
+ * order that ids, sizes and types set (no float atomics: the same bits on every run, wherever
+ * the tensors lie) and rounded once.  accumulate = 0: every row of dw (contiguous) is written,
+ * zeros where no id names it; accumulate = 1: the sums are added to dw's named rows (dwstride >= D
+ * elements apart, not in g's memory), the others are neither read nor written.  Padding ids take
  * no part.  Workspace: hgsr_embed_bwd_ws_bytes (any contents). */
 size_t hgsr_embed_bwd_ws_bytes(int64_t V, int64_t n, int64_t D);
 int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, int gtype, int64_t gstride, const void* ids,
@@ -621,9 +622,10 @@ int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, int gtype, in
  * (scales + c sstride), group = 16, 32, 64 or 128 columns.  With top = 127 (HGSR_INT8) or 448
  * (HGSR_E4M3: 4-bit exponent, 3-bit mantissa, no infinities), a row x is held as
  *   s = max(max |x| over the group * (1 / top), 2^-100),  code = x / s rounded to nearest, ties to
- * even -- s in f32, its product with the f32 number 1 / top rounded once, the quotient exact; a group that holds a NaN or an infinity has s = NaN and codes 0, so
- * it reads back as NaN.  A row whose slot lies outside [0, capacity) is left out; where a slot
- * is named twice, the last of its rows stays.  slots = NULL: row i goes to slot i (n <= capacity).
+ * even -- s in f32, its product with the f32 number 1 / top rounded once, the quotient exact;
+ * a group that holds a NaN or an infinity has s = NaN and codes 0, so it reads back as NaN.  A
+ * row whose slot lies outside [0, capacity) is left out; where a slot is named twice, the last
+ * of its rows stays.  slots = NULL: row i goes to slot i (n <= capacity).
  * Workspace: hgsr_rowcache_write_ws_bytes (any contents; 0 without slots). */
 enum { HGSR_INT8 = 0, HGSR_E4M3 = 1 };
 size_t hgsr_rowcache_write_ws_bytes(int64_t capacity, int64_t n, int has_slots);

@@ -171,6 +171,23 @@ def test_strides_and_shapes():
     assert torch.equal(E.embedding(every, skip.clamp(0, 19)), every[:1].expand(skip.numel(), 45))
 
 
+@pytest.mark.parametrize("V,n,D", [(40, 300, 24), (3, 4000, 16), (500, 9000, 40), (4000, 40_000, 16), (900, 2000, 1032)])
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_bits_do_not_depend_on_where_tensors_lie(V, n, D, t):
+    """The same values at every element offset and row stride: the same sums, bit for bit."""
+    ids = make_ids("mixed", V, n, n).to(DEV)
+    g = torch.randn(n, D, generator=gen(V)).to(t).to(DEV)
+    w = torch.randn(V, D, generator=gen(n)).to(t).to(DEV)
+    want, rows, base = E.embedding_grad(g, ids, V, 0.3), E.embedding(w, ids, 0.3), E.embedding_grad(g, ids, V, 0.3, out=w.clone())
+    for off in (1, 2, 3, 5):
+        for extra in (0, 1, 6):
+            place = lambda x: torch.empty(x.shape[0] * (D + extra) + off, dtype=t, device=DEV)[off:].view(x.shape[0], -1)[:, :D]
+            g1, w1, o1 = place(g).copy_(g), place(w).copy_(w), place(w).copy_(w)
+            assert torch.equal(E.embedding_grad(g1, ids, V, 0.3), want)
+            assert torch.equal(E.embedding(w1, ids, 0.3), rows)
+            assert torch.equal(E.embedding_grad(g1, ids, V, 0.3, out=o1), base)
+
+
 def test_empty():
     w = torch.zeros(4, 3, device=DEV)
     e = torch.empty(0, dtype=torch.int64, device=DEV)
