@@ -214,22 +214,32 @@ __global__ __launch_bounds__(1024) void sort_bucket_kernel(const BucketArgs<I> a
         // the range once more, its entries into global memory in order: done if they are one id's
         uint2* src = a.passes & 1 ? tmp : out;
         uint32_t filled = 0, lowest = ~0u, highest = 0;
-        for (uint32_t j0 = 0; j0 < n; j0 += 1024) {
-            const uint32_t i = j0 + tid, k = i < n ? a.ids.get(i, a.V) : ~0u;
-            const bool in = k != ~0u && k >> a.shift == bucket;
-            const uint64_t b = __ballot(in);
-            if (lane == 0) wsum[0][w] = __popcll(b);
+        for (uint32_t j0 = 0; j0 < n; j0 += kBucketKeep) {
+            const uint32_t base = j0 + w * kBucketRounds * 64 + lane;
+            uint32_t k[kBucketRounds], mine = 0;
+#pragma unroll
+            for (int r = 0; r < kBucketRounds; ++r) k[r] = base + r * 64 < n ? a.ids.get(base + r * 64, a.V) : ~0u;
+#pragma unroll
+            for (int r = 0; r < kBucketRounds; ++r)
+                mine += __popcll(__ballot(k[r] >> a.shift == bucket && k[r] != ~0u));
+            if (lane == 0) wsum[0][w] = mine;
             __syncthreads();
-            uint32_t at = filled + __popcll(b & below(lane));
+            uint32_t at = filled;
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
                 if (q < w) at += wsum[0][q];
                 filled += wsum[0][q];
             }
-            if (in) {
-                src[at] = make_uint2(k, i);
-                lowest = min(lowest, k);
-                highest = max(highest, k);
+#pragma unroll
+            for (int r = 0; r < kBucketRounds; ++r) {
+                const bool in = k[r] >> a.shift == bucket && k[r] != ~0u;
+                const uint64_t b = __ballot(in);
+                if (in) {
+                    src[at + __popcll(b & below(lane))] = make_uint2(k[r], base + r * 64);
+                    lowest = min(lowest, k[r]);
+                    highest = max(highest, k[r]);
+                }
+                at += __popcll(b);
             }
             __syncthreads();
         }
@@ -260,14 +270,21 @@ __global__ __launch_bounds__(1024) void sort_bucket_kernel(const BucketArgs<I> a
             uint2* dst = src == out ? tmp : out;
             for (uint32_t b = tid; b < 16 * bins; b += 1024) cnt[b >> a.bits][b & (bins - 1)] = 0;
             __syncthreads();
+#pragma unroll 8
             for (uint32_t i = i0 + lane; i < i1; i += 64) atomicAdd(&cnt[w][(src[i].x >> sh) & (bins - 1)], 1u);
             __syncthreads();
             digit_places(cnt, wsum[0], bins);
-            for (uint32_t i = i0; i < i1; i += 64) {
-                const bool on = i + lane < i1;
-                const uint2 e = src[on ? i + lane : i];
-                const uint32_t to = take_places(cnt[w], (e.x >> sh) & (bins - 1), on, a.bits, lane);
-                if (on) dst[to] = e;
+            for (uint32_t i = i0; i < i1; i += 4 * 64) {
+                uint2 e[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) e[r] = src[min(i + r * 64 + lane, i1 - 1)];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (i + r * 64 < i1) {
+                        const bool on = i + r * 64 + lane < i1;
+                        const uint32_t to = take_places(cnt[w], (e[r].x >> sh) & (bins - 1), on, a.bits, lane);
+                        if (on) dst[to] = e[r];
+                    }
             }
             __syncthreads();
             src = dst;

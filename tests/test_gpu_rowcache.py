@@ -146,17 +146,19 @@ def test_extreme_rows(fmt):
     assert y[6, :32].isnan().all() and float(y[6, 40]) == 2.0
 
 
-@pytest.mark.parametrize("n", [2, 70, 1000, 1100, 5000, 60_000])
-def test_repeated_and_outside_slots(n):
+@pytest.mark.parametrize("n,cap", [(2, 4), (70, 23), (1000, 333), (1024, 100), (1025, 100), (1100, 4), (5000, 1666),
+                                   (16_385, 16_384), (40_000, 16_385), (60_000, 20_000), (60_000, 7),
+                                   (33_000, 16_384), (3000, 4_000_000)])
+def test_repeated_and_outside_slots(n, cap):
     """The last row of a slot stays, rows outside the cache are left out, other slots keep what they hold."""
-    cap, D = max(4, n // 3), 32
+    D = 32
     x = torch.randn(n, D, generator=gen(n))
     slots = torch.randint(-2, cap + 2, (n,), generator=gen(n + 1))
     slots[slots == 1] = 0  # slot 1 is not named
     if n > 2:
         slots[-2:] = cap - 1
     c = R.rowcache_alloc(cap, D, "int8", 32, DEV)
-    base = torch.randn(cap, D, generator=gen(n + 2))
+    base = torch.randn(min(cap, 70_000), D, generator=gen(n + 2)).repeat(-(-cap // 70_000), 1)[:cap]
     R.rowcache_write(c, base.to(DEV))
     R.rowcache_write(c, x.to(DEV), slots.to(DEV))
     final = base.clone()
