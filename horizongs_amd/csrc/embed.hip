@@ -15,7 +15,8 @@
 // Forms, by the number of ids n, of rows V and the columns per lane (bwd_plan):
 //   n <= 1,024               one launch, a workgroup per id                       (600 x 2048: 9 us)
 //   V * columns <= 128       tables of sums in LDS, no sort     (500k x 32 f32, 16 rows: 20 us)
-//   n <= 32,768              sorted by ranges of ids, one launch   (16k x 2048 bf16, 65,536 rows: 68 us)
+//   n <= 32,768 (16,384 if V < 2048)
+//                            sorted by ranges of ids, one launch   (16k x 2048 bf16, 65,536 rows: 68 us)
 //   more                     radix sort           (500k x 32 f32 in order, a million rows: 52 us)
 // The last two are within 1.35 of what the same bytes take as a large copy.
 #include "rows.h"
@@ -106,13 +107,16 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {  // inclus
     return v;
 }
 
-// Up to kBucketMost entries: one launch.  The ids are cut into up to 256 ranges, a workgroup each: it
+// Up to 32,768 entries: one launch.  The ids are cut into up to 256 ranges, a workgroup each: it
 // reads all ids, keeps the positions of its own in LDS (in order) and counts the smaller ones, which
 // is where its part of the list starts; then it sorts what it kept by the ids' remaining bits.  A
 // range that does not fit (an id that half of the entries name) is sorted in global memory.
 // (One workgroup for all: 42 us at 16,384 entries, LDS-bound; counting, for each entry, the ones
 // before it: 36 us of the whole chip; this: 14.)
-constexpr int kBucketMost = 32768;
+// Up to where: 24,000 rows of 32 floats into 65,536 rows 25 us, 40 by the radix sort's two passes (53 and
+// 42 if half of the ids are one).  Up to 2,047 rows that sort has one pass: 24,000 into 404 25 us by
+// either (48 and 26), 10,000 into 404 17 and 24 (22 and 26).
+constexpr int kBucketMost = 32768, kBucketMostOfOne = 16384;
 constexpr int kBucketKeep = 8192;  // positions that a workgroup keeps
 constexpr int kBucketRounds = kBucketKeep / 1024;
 constexpr int kBucketLog = 8;
@@ -354,9 +358,8 @@ __global__ __launch_bounds__(1024) void sort_bucket_kernel(const BucketArgs<I> a
 }
 
 // More: digits of up to 11 bits, per pass three launches: the tiles' digit counts, their prefix over
-// the tiles, a stable scatter.  The first pass also notes whether the
-// ids ascend already (a compacted index does): the rest of the sort then ends at once, and the
-// sums read the ids themselves.
+// the tiles, a stable scatter.  The first pass also notes whether the ids ascend already (a compacted
+// index does): the rest of the sort then ends at once, and the sums read the ids themselves.
 constexpr int kSortRounds = 8;
 constexpr int kSortTile = 256 * kSortRounds;  // entries per workgroup: 4 waves x 8 rounds x 64 lanes
 constexpr int kSortBits = 11;
@@ -610,7 +613,8 @@ __device__ __forceinline__ void sum_subgroups(Vec<float, VEC>* part, float* acc,
 
 // ---- few entries: one launch, a workgroup per entry.  The first of the entries that name a row
 // sums them all (each subgroup every NS-th of them, joined through LDS); other workgroups store the
-// zeros of the rows that no id names.
+// zeros of the rows that no id names.  1,000 rows of 2048 bf16: 12 us, 16 by the sort; 25 if they are all
+// one row's (72 with a comparison around each of the eight loads, which then wait for one another).
 constexpr int kFewMost = 1024;
 constexpr int kFewRows = 1024;  // rows per zeroing workgroup, at most
 
@@ -665,15 +669,16 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
     float acc[VEC] = {};
     if (on) {
         const GT* g = static_cast<const GT*>(a.g) + col;
-        for (uint32_t j = s; j < m; j += 8 * NS) {
+        uint32_t j = s;
+        for (; j + 7 * NS < m; j += 8 * NS) {
             Vec<GT, VEC> x[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (j + u * NS < m) x[u] = load_vec<GT, VEC>(g + (int64_t)match[j + u * NS] * a.gstride);
+            for (int u = 0; u < 8; ++u) x[u] = load_vec<GT, VEC>(g + (int64_t)match[j + u * NS] * a.gstride);
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (j + u * NS < m) add_vec<GT, VEC>(acc, x[u]);
+            for (int u = 0; u < 8; ++u) add_vec<GT, VEC>(acc, x[u]);
         }
+#pragma unroll 4
+        for (; j < m; j += NS) add_vec<GT, VEC>(acc, load_vec<GT, VEC>(g + (int64_t)match[j] * a.gstride));
     }
     sum_subgroups<VEC>(part, acc, L, m < (uint32_t)NS ? (int)m : NS);
     if (s == 0 && on) put_row<OT, VEC>(a, v, c, acc);
@@ -681,7 +686,7 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
 
 // ---- few rows: no sort.  Every subgroup keeps a table of sums in LDS, its own, so a workgroup's
 // entries are read once and in order; the subgroups' and then the workgroups' tables are added.
-// 500k ids of rows of 32 floats: 16 rows 20.8 us (sorted: 37.8), 32 rows 28.6 (sorted: 37.6).
+// 500k ids of rows of 32 floats: 16 rows 20.8 us (sorted: 37.8), 32 rows 25.2 (sorted: 37.6).
 constexpr int kTableMost = 128;  // V * VEC: 128 KB of LDS
 
 template <typename GT, typename I, int VEC>
@@ -983,7 +988,8 @@ static BwdPlan bwd_plan(int64_t V, int64_t n, int64_t D, int vec) {
         o += align256(b);
         return at;
     };
-    p.form = n <= kFewMost ? kFew : V * vec <= kTableMost ? kTable : n <= kBucketMost ? kBucket : kRadix;
+    const int64_t bucket_most = V >> kSortBits ? kBucketMost : kBucketMostOfOne;
+    p.form = n <= kFewMost ? kFew : V * vec <= kTableMost ? kTable : n <= bucket_most ? kBucket : kRadix;
     if (p.form == kTable) {
         int64_t blocks = (V * vec > 64 ? 256 : 512) / p.slabs;  // as many as the tables leave room for
         if (blocks < 1) blocks = 1;

@@ -129,7 +129,8 @@ def test_grad(V, n, D, gt, ot):
     (600, 16_384, 8, "one"), (1 << 20, 16_000, 8, "mixed"), (200, 5000, 100, "uniform"),
     (90, 32_768, 12, "uniform"), (90, 32_769, 12, "uniform"), (1 << 20, 30_000, 8, "mixed"), (1 << 20, 60_000, 8, "mixed"), (1 << 20, 8193, 8, "one"),
     (300, 8192, 24, "mixed"), (300, 8193, 24, "mixed"), (300, 1024, 2048, "one"), (300, 1025, 2048, "one"),
-    (200_000_000, 30_000, 1, "mixed")])
+    (200_000_000, 30_000, 1, "mixed"), (2047, 16_384, 20, "mixed"), (2047, 16_385, 20, "mixed"),
+    (2048, 16_385, 20, "mixed"), (2048, 32_768, 20, "one"), (1600, 1000, 2048, "mixed"), (1600, 1021, 520, "one")])
 def test_grad_of_whole_numbers_is_exact(V, n, D, kind):
     ids = make_ids(kind, V, n, n).to(DEV)
     g = torch.randint(-8, 9, (n, D), generator=gen(V)).to(DEV)
@@ -367,3 +368,15 @@ def test_module():
     assert torch.equal(out, m.embedding.weight[i] * 2) and torch.equal(m.mean(), m.embedding.weight.mean(0))
     out.sum().backward()
     assert m.embedding.weight.grad[3].eq(4).all() and m.embedding.weight.grad[1].eq(0).all()
+
+
+def test_gradient_by_itself_is_differentiable():
+    V, n, D = 40, 90, 12
+    g = torch.randn(3, 30, D, generator=gen(0)).to(DEV).requires_grad_(True)
+    ids = make_ids("padded", V, n, 3).reshape(3, 30).to(DEV)
+    c = torch.randn(V, D, generator=gen(1)).to(DEV)
+    dw = E.embedding_grad(g, ids, V, 0.5)
+    with torch.no_grad():
+        assert torch.equal(dw, E.embedding_grad(g, ids, V, 0.5))
+    (dw * c).sum().backward()
+    assert torch.equal(g.grad.cpu().double(), want_lookup(c.cpu(), ids.cpu(), 0.5))
