@@ -160,10 +160,10 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
     """The lookup's gradient by itself: dw[v] = scale * sum of grad's rows whose id is v.
 
     grad [*ids.shape, D]; returns dw [num_rows, D] in `dtype` (default: grad's), zeros in rows that no
-    id names.  With out [num_rows, D] (contiguous columns, rows that do not overlap) the sums are added
+    id names, differentiable in grad.  With out [num_rows, D] (contiguous columns, rows that do not overlap) the sums are added
     to its named rows instead -- each row's sum and its old value are added in f32 and rounded once,
     the other rows are left as they are -- and out, which must not share memory with grad, is
-    returned."""
+    returned; nothing is differentiated through that."""
     type_code(grad.dtype)
     check_ids(ids)
     if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
@@ -175,6 +175,8 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
         dtype = grad.dtype if dtype is None else dtype
         type_code(dtype)
         index = check_device(grad, ids)
+        if D and grad.requires_grad and torch.is_grad_enabled():
+            return _EmbeddingGrad.apply(grad, flat_ids(ids), (num_rows, D), dtype, float(scale), index)
         out, accumulate = grad.new_empty((num_rows, D), dtype=dtype), 0
     else:
         type_code(out.dtype)
@@ -183,6 +185,8 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
                              f"{dtype or 'its type'}")
         if row_stride(out, "out") < D:
             raise ValueError("hgsr: the rows of out overlap")
+        if torch.is_grad_enabled() and (grad.requires_grad or out.requires_grad):
+            raise NotImplementedError("hgsr: sums added to out are not differentiable (torch.no_grad())")
         index, accumulate = check_device(grad, ids, out), 1
     g = rows_view(grad, D, "grad") if D else grad
     return _grad(g, flat_ids(ids), out, float(scale), accumulate, index)

@@ -36,6 +36,12 @@ def test_refused_arguments(call, match):
         call()
 
 
+def test_sums_added_to_a_table_are_not_differentiable():
+    for g, out in ((G, torch.zeros(5, 4, requires_grad=True)), (G.clone().requires_grad_(True), torch.zeros(5, 4))):
+        with pytest.raises(NotImplementedError, match="not differentiable"):
+            E.embedding_grad(g, I, 5, out=out)
+
+
 def test_cpu_tensors_are_refused():
     c = R.rowcache_alloc(5, 4, device="cpu")
     for call in (lambda: E.embedding(W, I), lambda: E.embedding_grad(G, I, 5), lambda: R.rowcache_write(c, G, I),
