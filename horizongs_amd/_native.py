@@ -98,7 +98,7 @@ _SIGS = {
     "hgsr_embed_fwd": (I, [I64, I64, I64, P, I, I64, P, I, I64, F, P, I, P]),
     "hgsr_embed_bwd_ws_bytes": (SZ, [I64, I64, I64]),
     "hgsr_embed_bwd": (I, [I64, I64, I64, P, I, I64, P, I, I64, F, P, I, I64, I, P, SZ, P]),
-    "hgsr_rowcache_write_ws_bytes": (SZ, [I64, I64, I]),
+    "hgsr_rowcache_write_ws_bytes": (SZ, [I64, I64, I64, I]),
     "hgsr_rowcache_write": (I, [I64, I64, I64, I, I, P, I, I64, P, I, I64, P, I64, P, I64, P, SZ, P]),
     "hgsr_rowcache_read": (I, [I64, I64, I64, I, I, P, I64, P, I64, P, I, I64, P, I, P]),
     "hgsr_timing_enable": (I, [I]),

@@ -30,6 +30,7 @@ struct CacheArgs {
     int64_t xstride;
     const int32_t* last;               // write: the last row of each named slot (nullable), unless
     const uint32_t* distinct;          // this is set: no slot is named twice
+    int tlog;                          // write of few rows: the table has 1 << tlog places
 };
 
 template <typename I>
@@ -118,12 +119,20 @@ __device__ __forceinline__ void decode4(uint32_t w, float* o) {
 
 // ------------------------------------------------------------------------------------- write
 
-// More than kFewSlots rows: `last` is the last row that names each slot.  Slots in strictly ascending
-// order (a compacted index, a chunk appended) cannot repeat: the first launch finds out tile by tile,
-// the second ends at once, and the write does not look.  Otherwise `last`, cleared by the first launch
-// where rows name it, is raised to their numbers by the second: by an atomic for every row (500k rows
-// of 32 floats into a million slots 58 us in all, 24 in order), or, up to 16,384 slots, of which each
-// may have many rows, by tiles of rows in LDS first (270k rows of 12 into 404: 16 us, 105 by atomics).
+// Few rows: no launch before the write, each of whose workgroups (4,096 columns) spends the time of n
+// inserts.  2,048 rows of 1024 bf16 9 us, 16 with the launches below; of 2048 9.4 and 16.3; of 4096 17.2
+// and 17.1; of 8192 30 and 23.
+constexpr int kFewSlots = 2048;
+constexpr int64_t kFewWork = 1ll << 33;  // n n D
+
+static bool few_slots(int64_t n, int64_t D) { return n <= kFewSlots && n * n * D <= kFewWork; }
+
+// More: `last` is the last row that names each slot.  Slots in strictly ascending order (a compacted
+// index, a chunk appended) cannot repeat: the first launch finds out tile by tile, the second ends at once,
+// and the write does not look.  Otherwise `last`, cleared by the first launch where rows name it, is raised
+// to their numbers by the second: by an atomic for every row (500k rows of 32 floats into a million slots
+// 58 us in all, 24 in order), or, up to 16,384 slots, of which each may have many rows, by tiles of rows in
+// LDS first (270k rows of 12 into 404: 16 us, 105 by atomics).
 constexpr int kSlotTile = 1024;
 constexpr int kFewCapacity = 16384;
 constexpr int kSlotWide = 16384;  // rows per workgroup of the LDS form
@@ -196,13 +205,13 @@ __global__ __launch_bounds__(256) void slot_last_each_kernel(uint32_t n, RowIds<
     }
 }
 
-// VEC consecutive columns per lane, fewer where the row ends.  FEW: no more than
-// kFewSlots rows, whose repeated slots are found here, by a group's lanes among the later rows.
-constexpr int kFewSlots = 1024;
-
+// VEC consecutive columns per lane, fewer where the row ends.  FEW: every workgroup finds the last row of
+// each slot itself, in a table in LDS with at least twice as many places as rows (a slot lies at the first
+// place from its hash on that no other slot holds).
 template <typename XT, typename I, int FMT, int VEC, bool FEW>
 __global__ __launch_bounds__(256) void rowcache_write_kernel(const CacheArgs<I> a) {
-    __shared__ uint32_t slots[FEW ? kFewSlots : 1];
+    __shared__ uint32_t key[FEW ? 2 * kFewSlots : 1];
+    __shared__ int32_t last[FEW ? 2 * kFewSlots : 1];
     // Narrow rows: an XCD's workgroups take consecutive ones, so that slots in order share its L2's lines
     // (500k rows of 32 floats 24.5 us, 25.3 without).  Wide ones share none (16k of 2048: 41.8, 43.1 with).
     const uint32_t c = (a.D < 128 ? xcd_remap(blockIdx.x, gridDim.x) : blockIdx.x) * 256 + threadIdx.x;
@@ -221,22 +230,43 @@ __global__ __launch_bounds__(256) void rowcache_write_kernel(const CacheArgs<I> 
 #pragma unroll
         for (int k = 0; k < VEC; ++k) x[k] = col + k < D ? (float)p[k] : 0.0f;
     }
-    if (FEW) {
-        for (uint32_t i = threadIdx.x; i < (uint32_t)a.n; i += 256) slots[i] = slot_of(a, i);
-        __syncthreads();
-    }
     bool on = col < D && slot < a.capacity;
-    if (!FEW && a.last && !*a.distinct && on) on = a.last[slot] == (int32_t)row;
+    if (FEW) {
+        constexpr uint32_t NONE = ~0u;
+        const uint32_t mask = (1u << a.tlog) - 1;
+        const auto home = [&](uint32_t v) { return (v * 0x9e3779b9u) >> (32 - a.tlog); };
+        for (uint32_t k = threadIdx.x; k <= mask; k += 256) {
+            key[k] = NONE;
+            last[k] = -1;
+        }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < (uint32_t)a.n; i += 256) {
+            const uint32_t v = slot_of(a, i);
+            if (v >= a.capacity) continue;
+            uint32_t h = home(v);
+            for (;;) {
+                const uint32_t old = atomicCAS(&key[h], NONE, v);
+                if (old == NONE || old == v) break;
+                h = (h + 1) & mask;
+            }
+            atomicMax(&last[h], (int32_t)i);
+        }
+        __syncthreads();
+        if (on) {
+            uint32_t h = home(slot);
+            while (key[h] != slot) h = (h + 1) & mask;
+            on = last[h] == (int32_t)row;
+        }
+    } else if (a.last && !*a.distinct && on) {
+        on = a.last[slot] == (int32_t)row;
+    }
     // the largest magnitude of the group as bits: infinities and NaN lie above every number
     const int lanes = a.group / VEC;  // a power of two, <= 8
     uint32_t m = 0;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) m = max(m, __float_as_uint(x[k]) & 0x7fffffffu);
-    if (FEW)  // a later row of the same slot: a mark above every magnitude
-        for (uint32_t j = (uint32_t)row + 1 + (threadIdx.x & (lanes - 1)); j < (uint32_t)a.n; j += lanes)
-            if (slots[j] == slot) m = 0x80000000u;
     for (int d = 1; d < lanes; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
-    if (!on || (FEW && m == 0x80000000u)) return;
+    if (!on) return;
     const bool finite = m < 0x7f800000u;
     const float per = FMT == HGSR_INT8 ? 1.0f / 127.0f : 1.0f / 448.0f;
     const float s = fmaxf(__uint_as_float(m) * per, kScaleFloor), inv = 1.0f / s;
@@ -313,7 +343,7 @@ template <bool WRITE, typename T, int FMT, int VEC, typename I>
 static void launch(const CacheArgs<I>& a, hipStream_t s) {
     const dim3 block(256), grid((a.chunks + 255) / 256);
     if constexpr (WRITE) {
-        if (a.slots.p && a.n > 1 && a.n <= kFewSlots)
+        if (a.slots.p && a.n > 1 && few_slots(a.n, a.D))
             hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, true>), grid, block, 0, s, a);
         else
             hipLaunchKernelGGL((rowcache_write_kernel<T, I, FMT, VEC, false>), grid, block, 0, s, a);
@@ -375,7 +405,8 @@ static void launch(const CacheCall& c, hipStream_t s) {
     a.slots = RowIds<I>{static_cast<const I*>(c.slots), c.slots_stride};
     a.x = c.x;
     a.xstride = c.xstride;
-    if (WRITE && c.slots && c.n > kFewSlots) {
+    while ((1ll << a.tlog) < 2 * c.n && a.tlog < 30) ++a.tlog;
+    if (WRITE && c.slots && !few_slots(c.n, c.D)) {
         const SlotWork w = slot_work(c.ws, c.n);
         const uint32_t n = (uint32_t)c.n, cap = a.capacity;
         hipLaunchKernelGGL((slot_check_kernel<I>), dim3(w.tiles), dim3(256), 0, s, n, a.slots, cap, w);
@@ -423,8 +454,8 @@ static int check_cache(const char* what, const CacheCall& c) {
     return HGSR_OK;
 }
 
-extern "C" size_t hgsr_rowcache_write_ws_bytes(int64_t capacity, int64_t n, int has_slots) {
-    if (!has_slots || n <= kFewSlots || capacity <= 0) return 0;
+extern "C" size_t hgsr_rowcache_write_ws_bytes(int64_t capacity, int64_t n, int64_t D, int has_slots) {
+    if (!has_slots || n <= 0 || capacity <= 0 || D < 1 || few_slots(n, D)) return 0;
     return align256(((size_t)(n + kSlotTile - 1) / kSlotTile + 1) * 4) + (size_t)capacity * sizeof(int32_t);
 }
 
@@ -437,7 +468,7 @@ extern "C" int hgsr_rowcache_write(int64_t capacity, int64_t n, int64_t D, int g
     if (int st = check_cache("rowcache_write", c)) return st;
     if (n == 0 || capacity == 0) return HGSR_OK;
     HGSR_REQUIRE(x && codes && scales, "rowcache_write: null pointer");
-    const size_t need = hgsr_rowcache_write_ws_bytes(capacity, n, slots != nullptr);
+    const size_t need = hgsr_rowcache_write_ws_bytes(capacity, n, D, slots != nullptr);
     if (need > ws_bytes || (need && !ws)) {
         set_error("rowcache_write: workspace of %zu bytes, %zu needed", ws ? ws_bytes : (size_t)0, need);
         return HGSR_EWORKSPACE;

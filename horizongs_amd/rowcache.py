@@ -94,7 +94,7 @@ def rowcache_write(cache, rows, slots=None):
         index = check_device(codes, scales, rows, slots)
     if n == 0 or capacity == 0:
         return
-    ws_b = N.size_query("hgsr_rowcache_write_ws_bytes", capacity, n, int(slots is not None))
+    ws_b = N.size_query("hgsr_rowcache_write_ws_bytes", capacity, n, dim, int(slots is not None))
     ws = torch.empty(ws_b, dtype=torch.uint8, device=codes.device) if ws_b else None
     N.call_on(index, "hgsr_rowcache_write", capacity, n, dim, group, _FORMATS[codes.dtype], rows.data_ptr(), xt, xs,
               *_slot_args(slots), codes.data_ptr(), cs, scales.data_ptr(), ss, ws.data_ptr() if ws_b else None, ws_b)

@@ -628,7 +628,7 @@ int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, int gtype, in
  * of its rows stays.  slots = NULL: row i goes to slot i (n <= capacity).
  * Workspace: hgsr_rowcache_write_ws_bytes (any contents; 0 without slots). */
 enum { HGSR_INT8 = 0, HGSR_E4M3 = 1 };
-size_t hgsr_rowcache_write_ws_bytes(int64_t capacity, int64_t n, int has_slots);
+size_t hgsr_rowcache_write_ws_bytes(int64_t capacity, int64_t n, int64_t D, int has_slots);
 int hgsr_rowcache_write(int64_t capacity, int64_t n, int64_t D, int group, int format, const void* x, int xtype,
                         int64_t xstride, const void* slots, int slots64, int64_t slots_stride, void* codes,
                         int64_t cstride, float* scales, int64_t sstride, void* ws, size_t ws_bytes,

@@ -178,6 +178,34 @@ def test_repeated_and_outside_slots(n, cap):
     assert torch.equal(c.codes[cap - 1].cpu().double(), torch.from_numpy(want_write(x[-1:].numpy(), "int8", 32)[0])[0])
 
 
+@pytest.mark.parametrize("n,D,group,kind", [(2048, 40, 16, "two"), (2049, 40, 16, "two"), (2048, 2048, 128, "two"),
+                                            (2048, 2064, 16, "two"), (700, 33_000, 64, "two"), (1000, 16, 16, "same place"),
+                                            (2048, 20, 32, "power"), (2048, 16, 16, "padded")])
+def test_last_rows_of_few(n, D, group, kind):
+    """Each slot named about twice, by rows of every width; slots that one hash sends to one place."""
+    cap = 1 << 22 if D < 32 else n
+    if kind == "same place":  # the last place of a table of 2^11, so that the search wraps around
+        v = np.arange(cap, dtype=np.uint64)
+        slots = torch.from_numpy(v[((v * 0x9e3779b9) & 0xffffffff) >> 21 == 2047][:n // 2].astype(np.int64)).repeat(2)
+    elif kind == "power":
+        slots = torch.arange(n // 2).repeat_interleave(2) << 11
+    else:
+        slots = torch.randint(0, n // 2, (n,), generator=gen(n + D))
+        if kind == "padded":
+            slots[::3] = -1
+    x = torch.randn(n, D, generator=gen(D))
+    c = R.rowcache_alloc(cap, D, "int8", group, DEV)
+    R.rowcache_write(c, x.to(DEV), slots.to(DEV))
+    last = {k: i for i, k in enumerate(slots.tolist()) if k >= 0}
+    at, rows = torch.tensor(list(last)), torch.tensor(list(last.values()))
+    q, s = want_write(x[rows].numpy(), "int8", group)
+    np.testing.assert_array_equal(c.codes[at.to(DEV)].cpu().numpy(), q)
+    np.testing.assert_array_equal(c.scales[at.to(DEV)].cpu().numpy(), s)
+    rest = torch.ones(cap, dtype=torch.bool, device=DEV)
+    rest[at.to(DEV)] = False
+    assert not c.scales[rest].any()  # no other slot was written
+
+
 @pytest.mark.parametrize("n", [1025, 2048, 2049, 30_000])
 @pytest.mark.parametrize("twice", [None, 0, 2047, -2])
 def test_slots_in_order(n, twice):
