@@ -588,6 +588,19 @@ __device__ __forceinline__ void put_row(const SumArgs<I>& a, uint32_t v, const C
         store_vec<OT, VEC>(p, o);
 }
 
+// a row that no id names: zeros whatever the scale
+template <typename OT, int VEC, bool STREAM = false, typename I>
+__device__ __forceinline__ void put_zeros(const SumArgs<I>& a, uint32_t v, const Cols<VEC>& c) {
+    OT* p = static_cast<OT*>(a.dw) + (int64_t)v * a.dwstride + c.col;
+    Vec<OT, VEC> o;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) o.v[k] = (OT)0.0f;
+    if (STREAM)
+        stream_vec<OT, VEC>(p, o);
+    else
+        store_vec<OT, VEC>(p, o);
+}
+
 template <typename T, int VEC>
 __device__ __forceinline__ void add_vec(float* acc, const Vec<T, VEC>& x) {
 #pragma unroll
@@ -641,9 +654,8 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
         for (int k = 0; k < PER; ++k)
             if (mine[k] < a.V && mine[k] >= r0 && mine[k] - r0 < a.rows) named[mine[k] - r0] = 1;
         __syncthreads();
-        const float z[VEC] = {};
         for (uint32_t k = s; k < a.rows && r0 + k < a.V; k += NS)
-            if (on && !named[k]) put_row<OT, VEC>(a, r0 + k, c, z);
+            if (on && !named[k]) put_zeros<OT, VEC>(a, r0 + k, c);
         return;
     }
     const uint32_t v = a.ids.get(blockIdx.x, a.V);
@@ -761,7 +773,11 @@ __global__ __launch_bounds__(1024) void embed_table_join_kernel(const SumArgs<I>
     }
     hit = __syncthreads_or(hit);
     sum_subgroups<VEC>(part, acc, L, NS);
-    if (s == 0 && on && (hit || !a.accumulate)) put_row<OT, VEC>(a, v, c, acc);
+    if (s != 0 || !on) return;
+    if (hit)
+        put_row<OT, VEC>(a, v, c, acc);
+    else if (!a.accumulate)
+        put_zeros<OT, VEC>(a, v, c);
 }
 
 // ---- the general form: every subgroup walks `run` consecutive entries of the sorted list, and a
@@ -908,9 +924,8 @@ __device__ __forceinline__ void zero_between(const SumArgs<I>& a, uint32_t r0) {
     }
     __syncthreads();
     const Cols<VEC> c(a.D, L, ln);
-    const float z[VEC] = {};
     for (uint32_t k = s; k < a.rows && r0 + k < a.V; k += NS)
-        if (c.on && !named[k]) put_row<OT, VEC, true>(a, r0 + k, c, z);
+        if (c.on && !named[k]) put_zeros<OT, VEC, true>(a, r0 + k, c);
 }
 
 // One workgroup per workgroup of the sums: if a run begins in it and goes on, its tail and the
@@ -1049,7 +1064,8 @@ static ZeroPart take_zeros(const ZeroPart& z, int k, int parts, uint32_t& blocks
     part.p = z.p + u0;
     part.units = u1 - u0;
     if (k) part.nedge[0] = part.nedge[1] = 0;
-    blocks = (uint32_t)((part.units + kZeroUnits - 1) / kZeroUnits);
+    const int64_t want = (part.units + kZeroUnits - 1) / kZeroUnits;
+    blocks = (uint32_t)(want < 1 << 20 ? want : 1 << 20);  // a launch holds fewer than 2^32 threads
     if (k == 0 && blocks == 0) blocks = 1;
     return part;
 }
@@ -1267,7 +1283,7 @@ extern "C" int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, in
     HGSR_REQUIRE(dw, "embed_bwd: null pointer");
     hipStream_t s = as_stream(stream);
     const size_t dw_bytes = (size_t)V * D * elem_size(dwtype);
-    HGSR_REQUIRE(dw_bytes / (kZeroUnits * 16) < (1ull << 30), "embed_bwd: table too large");
+    HGSR_REQUIRE(accumulate || dw_bytes >> 38 == 0, "embed_bwd: a dense gradient of %zu bytes: less than 2^38", dw_bytes);
     if (n == 0) {
         if (!accumulate) {
             uint32_t zb;
@@ -1284,6 +1300,8 @@ extern "C" int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, in
         set_error("embed_bwd: workspace of %zu bytes, %zu needed", ws ? ws_bytes : (size_t)0, p.bytes);
         return HGSR_EWORKSPACE;
     }
+    HGSR_REQUIRE(p.blocks < (1u << 24), "embed_bwd: %lld ids of rows of %lld: too many for a launch", (long long)n,
+                 (long long)D);
     char* w = static_cast<char*>(ws);
     auto run = [&](auto none) {
         SumArgs<decltype(none)> a{};

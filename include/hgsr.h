@@ -610,10 +610,10 @@ int hgsr_embed_fwd(int64_t V, int64_t n, int64_t D, const void* weight, int wtyp
                    int ids64, int64_t ids_stride, float scale, void* out, int otype, hgsr_stream_t stream);
 /* Its gradient, dw[v, :] = scale * sum over i with ids[i] = v of g[i, :], summed in f32 in an
  * order that ids, sizes and types set (no float atomics: the same bits on every run, wherever
- * the tensors lie) and rounded once.  accumulate = 0: every row of dw (contiguous) is written,
- * zeros where no id names it; accumulate = 1: the sums are added to dw's named rows (dwstride >= D
- * elements apart, not in g's memory), the others are neither read nor written.  Padding ids take
- * no part.  Workspace: hgsr_embed_bwd_ws_bytes (any contents). */
+ * the tensors lie) and rounded once.  accumulate = 0: every row of dw (contiguous, less than 2^38
+ * bytes) is written, zeros where no id names it; accumulate = 1: the sums are added to dw's named
+ * rows (dwstride >= D elements apart, not in g's memory), the others are neither read nor written.
+ * Padding ids take no part.  Workspace: hgsr_embed_bwd_ws_bytes (any contents). */
 size_t hgsr_embed_bwd_ws_bytes(int64_t V, int64_t n, int64_t D);
 int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, int gtype, int64_t gstride, const void* ids,
                    int ids64, int64_t ids_stride, float scale, void* dw, int dwtype, int64_t dwstride, int accumulate,

@@ -221,6 +221,19 @@ def test_non_finite_values_stay_in_their_rows():
         assert dw[0].eq(1).all() and dw[1].isnan().all() and dw[2].eq(2).all() and dw[3].eq(0).all()
 
 
+@pytest.mark.parametrize("V,n,D,kind", [(40, 30, 8, "uniform"), (6, 3000, 8, "one"), (900, 3000, 8, "uniform"),
+                                        (60_000, 50_000, 8, "uniform"), (60_000, 50_000, 8, "sorted")])
+def test_rows_without_ids_are_zeros_for_every_scale(V, n, D, kind):
+    ids = make_ids(kind, V, n, 1)
+    rest = torch.ones(V, dtype=torch.bool)
+    rest[ids] = False
+    for scale in (-2.0, float("inf"), float("nan")):
+        dw = E.embedding_grad(torch.ones(n, D, device=DEV), ids.to(DEV), V, scale).cpu()
+        assert rest.any() and not dw[rest].view(torch.int32).any()
+        assert torch.equal(dw[~rest].isfinite(), torch.full_like(dw[~rest], np.isfinite(scale)).bool())
+        assert E.embedding(torch.ones(V, D, device=DEV), torch.tensor([-1, V], device=DEV), scale).eq(0).all()
+
+
 def test_autograd_and_differences():
     V, n, D, scale = 30, 50, 12, 0.5
     w = torch.randn(V, D, generator=gen(0)).to(DEV).requires_grad_(True)
@@ -348,6 +361,23 @@ def test_table_beyond_2_31_elements():
     assert torch.equal(dense[ids[:5]], w[ids[:5]])
     dense[ids[:5]] = 0
     assert not dense.any()
+
+
+@pytest.mark.parametrize("n", [500, 3000, 40_000])
+def test_table_of_140_gib(n):
+    """More zeros than the threads of one launch can store a piece each."""
+    V, D = 560_000, 1 << 16
+    if torch.cuda.mem_get_info()[0] < 180 << 30:
+        pytest.skip("180 GiB of free memory are needed")
+    ids = torch.randint(0, V, (n,), generator=gen(n)).to(DEV)
+    ids[:2] = torch.tensor([0, V - 1], device=DEV)
+    dw = E.embedding_grad(torch.ones(1, D, device=DEV).expand(n, D), ids, V)
+    count = torch.bincount(ids, minlength=V).float()
+    for r in range(0, V, 20_000):
+        part = dw[r:r + 20_000]
+        assert torch.equal(part.amin(1), count[r:r + 20_000]) and torch.equal(part.amax(1), count[r:r + 20_000])
+    del dw, part
+    torch.cuda.empty_cache()
 
 
 def test_rows_beyond_2_31_elements():

@@ -93,6 +93,8 @@ def test_c_entries_refuse_before_any_launch():
     refused(lib.hgsr_embed_bwd(4, 1, 4, f, 0, 4, f, 0, 1, 1.0, t, 0, 3, 0, f, 1 << 20, None), "stride")
     refused(lib.hgsr_embed_bwd(4, 1, 4, f, 0, 4, f, 0, 1, 1.0, None, 0, 4, 0, f, 1 << 20, None), "null")
     refused(lib.hgsr_embed_bwd(4, 1, 4, f, 0, 4, f, 0, 1, 1.0, t, 0, 5, 0, f, 1 << 20, None), "contiguous")
+    refused(lib.hgsr_embed_bwd(1 << 30, 1, 64, f, 0, 4, f, 0, 1, 1.0, t, 0, 64, 0, f, 1 << 20, None), "dense gradient")
+    refused(lib.hgsr_embed_bwd(1 << 20, 1 << 30, 2048, f, 0, 0, f, 0, 1, 1.0, t, 0, 2048, 0, f, 1 << 50, None), "too many")
     for V, n in ((4, 2000), (1000, 2000), (1000, 100_000)):  # each form that keeps a workspace
         need = lib.hgsr_embed_bwd_ws_bytes(V, n, 4)
         refused(lib.hgsr_embed_bwd(V, n, 4, f, 0, 4, f, 0, 1, 1.0, t, 0, 4, 0, f, 0, None), "workspace", -3)
@@ -104,7 +106,8 @@ def test_c_entries_refuse_before_any_launch():
     refused(lib.hgsr_rowcache_write(4, 1, 4, 32, 2, f, 0, 4, None, 0, 1, *cache, None, 0, None), "format")
     refused(lib.hgsr_rowcache_write(4, 5, 4, 32, 0, f, 0, 4, None, 0, 1, *cache, None, 0, None), "slots")
     refused(lib.hgsr_rowcache_write(4, 5000, 4, 32, 0, f, 0, 4, f, 0, 1, *cache, None, 0, None), "workspace", -3)
-    assert lib.hgsr_rowcache_write_ws_bytes(9, 5000, 1) >= 36 and lib.hgsr_rowcache_write_ws_bytes(9, 5000, 0) == 0
+    ws = lib.hgsr_rowcache_write_ws_bytes
+    assert ws(9, 5000, 4, 1) >= 36 and ws(9, 5000, 4, 0) == 0 and ws(9, 2048, 4, 1) == 0 and ws(9, 2048, 1 << 20, 1) >= 36
     refused(lib.hgsr_rowcache_read(4, 1, 40, 32, 0, f, 40, f, 1, None, 0, 1, t, 0, None), "stride")
     refused(lib.hgsr_rowcache_read(4, 1, 4, 32, 0, f, 4, f, 1, None, 0, 1, None, 0, None), "null")
     # nothing to do: no launch, no error
