@@ -15,7 +15,7 @@
 // Forms, by the number of ids n, of rows V and the columns per lane (bwd_plan):
 //   n <= 1,024               one launch, a workgroup per id                       (600 x 2048: 9 us)
 //   V * columns <= 128       tables of sums in LDS, no sort     (500k x 32 f32, 16 rows: 20 us)
-//   n <= 32,768 (16,384 if V < 2048)
+//   n <= 24,576 (16,384 if V < 2048)
 //                            sorted by ranges of ids, one launch   (16k x 2048 bf16, 65,536 rows: 68 us)
 //   more                     radix sort           (500k x 32 f32 in order, a million rows: 52 us)
 // The last two are within 1.35 of what the same bytes take as a large copy.
@@ -107,16 +107,17 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {  // inclus
     return v;
 }
 
-// Up to 32,768 entries: one launch.  The ids are cut into up to 256 ranges, a workgroup each: it
+// Up to 24,576 entries: one launch.  The ids are cut into up to 256 ranges, a workgroup each: it
 // reads all ids, keeps the positions of its own in LDS (in order) and counts the smaller ones, which
 // is where its part of the list starts; then it sorts what it kept by the ids' remaining bits.  A
 // range that does not fit (an id that half of the entries name) is sorted in global memory.
 // (One workgroup for all: 42 us at 16,384 entries, LDS-bound; counting, for each entry, the ones
 // before it: 36 us of the whole chip; this: 14.)
-// Up to where: 24,000 rows of 32 floats into 65,536 rows 25 us, 40 by the radix sort's two passes (53 and
-// 42 if half of the ids are one).  Up to 2,047 rows that sort has one pass: 24,000 into 404 25 us by
-// either (48 and 26), 10,000 into 404 17 and 24 (22 and 26).
-constexpr int kBucketMost = 32768, kBucketMostOfOne = 16384;
+// Up to where: 24,000 ids of 65,536 rows of 64 floats 25 us if they are spread evenly, 46 if the low ones are
+// frequent (Zipf), by the radix sort's two passes 40 and 41; 32,000 ids 36 and 57, 40 and 42.  Up to 2,047
+// rows that sort has one pass: 24,000 of 404 rows 25 us by either, 48 and 26 if half of the ids are one;
+// 10,000 of 404 17 and 24, 22 and 26.
+constexpr int kBucketMost = 24576, kBucketMostOfOne = 16384;
 constexpr int kBucketKeep = 8192;  // positions that a workgroup keeps
 constexpr int kBucketRounds = kBucketKeep / 1024;
 constexpr int kBucketLog = 8;

@@ -130,7 +130,8 @@ def test_grad(V, n, D, gt, ot):
     (90, 32_768, 12, "uniform"), (90, 32_769, 12, "uniform"), (1 << 20, 30_000, 8, "mixed"), (1 << 20, 60_000, 8, "mixed"), (1 << 20, 8193, 8, "one"),
     (300, 8192, 24, "mixed"), (300, 8193, 24, "mixed"), (300, 1024, 2048, "one"), (300, 1025, 2048, "one"),
     (200_000_000, 30_000, 1, "mixed"), (2047, 16_384, 20, "mixed"), (2047, 16_385, 20, "mixed"),
-    (2048, 16_385, 20, "mixed"), (2048, 32_768, 20, "one"), (1600, 1000, 2048, "mixed"), (1600, 1021, 520, "one")])
+    (2048, 16_385, 20, "mixed"), (2048, 24_576, 20, "one"), (2048, 24_577, 20, "one"), (100_000, 24_000, 20, "mixed"),
+    (1600, 1000, 2048, "mixed"), (1600, 1021, 520, "one")])
 def test_grad_of_whole_numbers_is_exact(V, n, D, kind):
     ids = make_ids(kind, V, n, n).to(DEV)
     g = torch.randint(-8, 9, (n, D), generator=gen(V)).to(DEV)
