@@ -557,8 +557,8 @@ struct Cols {
     int64_t col;
     int skip;
     bool on;
-    __device__ __forceinline__ Cols(int64_t D, int lanes, int ln) {
-        const int64_t c = ((int64_t)blockIdx.y * lanes + ln) * VEC;
+    __device__ __forceinline__ Cols(int64_t D, int lanes, int ln, uint32_t slab) {
+        const int64_t c = ((int64_t)slab * lanes + ln) * VEC;
         on = c < D;
         col = c < D - VEC ? c : D - VEC;
         skip = on ? (int)(c - col) : 0;
@@ -641,7 +641,7 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
     __shared__ uint8_t named[kFewRows];
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const int L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
-    const Cols<VEC> c(a.D, L, ln);
+    const Cols<VEC> c(a.D, L, ln, blockIdx.y);
     const int64_t col = c.col;
     const bool on = c.on;
     uint32_t mine[PER];
@@ -708,7 +708,7 @@ __global__ __launch_bounds__(256) void embed_table_kernel(const SumArgs<I> a) {
     Vec<float, VEC>* tab = reinterpret_cast<Vec<float, VEC>*>(smem);  // [V][256]
     __shared__ uint8_t named[kTableMost];
     const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
-    const Cols<VEC> c(a.D, L, ln);
+    const Cols<VEC> c(a.D, L, ln, blockIdx.y);
     const int64_t col = c.col;
     const bool on = c.on;
     Vec<float, VEC> zero;
@@ -757,7 +757,7 @@ __global__ __launch_bounds__(1024) void embed_table_join_kernel(const SumArgs<I>
     __shared__ Vec<float, VEC> part[1024];
     const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 1024 / L;
     const uint32_t v = blockIdx.x, share = (a.blocks + NS - 1) / NS;
-    const Cols<VEC> c(a.D, L, ln);
+    const Cols<VEC> c(a.D, L, ln, blockIdx.y);
     const int64_t col = c.col;
     const bool on = c.on;
     float acc[VEC] = {};
@@ -800,7 +800,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs<I> a) {
     const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
     const uint32_t E = NS * a.run, block = xcd_remap(blockIdx.x, gridDim.x);
     uint32_t* pos = key + E + 2;
-    const Cols<VEC> c(a.D, L, ln);
+    const Cols<VEC> c(a.D, L, ln, blockIdx.y);
     const int64_t col = c.col;
     const bool on = c.on, asc = a.ascend && *a.ascend;
     constexpr uint32_t NONE = ~0u;
@@ -924,60 +924,104 @@ __device__ __forceinline__ void zero_between(const SumArgs<I>& a, uint32_t r0) {
         }
     }
     __syncthreads();
-    const Cols<VEC> c(a.D, L, ln);
+    const Cols<VEC> c(a.D, L, ln, blockIdx.y);
     for (uint32_t k = s; k < a.rows && r0 + k < a.V; k += NS)
         if (c.on && !named[k]) put_zeros<OT, VEC, true>(a, r0 + k, c);
 }
 
-// One workgroup per workgroup of the sums: if a run begins in it and goes on, its tail and the
-// heads of the workgroups it reaches into, each subgroup a consecutive share, joined through LDS.
-template <typename OT, typename I, int VEC>
-__global__ __launch_bounds__(256) void embed_join_kernel(const SumArgs<I> a) {
+// The last workgroup whose first entry is v's, lo's being one (the list is sorted); by a whole wave.
+template <typename I>
+__device__ __forceinline__ uint32_t last_with(const SumArgs<I>& a, bool asc, uint32_t E, uint32_t v, uint32_t lo) {
+    uint32_t hi = a.blocks;  // v's at lo, not at hi
+    const uint32_t lane = threadIdx.x & 63;
+    while (hi - lo > 1) {
+        const uint32_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
+        const uint32_t k = __popcll(__ballot(at < hi && sorted_id(a, asc, at * E) == v));  // these come first
+        hi = min(hi, lo + (k + 1) * step);
+        lo += k * step;
+    }
+    return lo;
+}
+
+// The sums of a run that begins in workgroup b and reaches into b + 1 .. b + m: b's tail and the others'
+// heads, each subgroup of the 256 / lanes a consecutive share, joined through LDS.
+template <typename OT, int VEC, typename I>
+__device__ __forceinline__ void join_run(const SumArgs<I>& a, uint32_t v, uint32_t b, uint32_t m, int L,
+                                         const Cols<VEC>& c) {
     __shared__ Vec<float, VEC> part[256];
-    __shared__ uint32_t s_last;
-    const int tid = threadIdx.x, L = a.lanes, s = tid / L, ln = tid & (L - 1), NS = 256 / L;
-    const bool asc = a.ascend && *a.ascend;
-    if (blockIdx.x >= a.blocks) {
-        if (asc) zero_between<OT, VEC>(a, (blockIdx.x - a.blocks) * a.rows);
-        return;
-    }
-    const uint32_t E = NS * a.run, b = blockIdx.x, i0 = b * E, i1 = i0 + E;
-    if (i1 >= a.n) return;
-    const uint32_t v = sorted_id(a, asc, i1), v1 = sorted_id(a, asc, i1 - 1), v0 = sorted_id(a, asc, b ? i0 - 1 : i1);
-    if (v >= a.V || v1 != v || (b && v0 == v)) return;
-    if (tid < 64) {  // the last workgroup whose first entry is v's (the list is sorted): 64 probes at a time
-        uint32_t lo = b + 1, hi = a.blocks;  // v's at lo, not at hi
-        while (hi - lo > 1) {
-            const uint32_t step = (hi - lo + 63) / 64, at = lo + (tid + 1) * step;
-            const uint64_t in = __ballot(at < hi && sorted_id(a, asc, at * E) == v);
-            const uint32_t k = __popcll(in);  // the probes that hold v come first
-            hi = min(hi, lo + (k + 1) * step);
-            lo += k * step;
-        }
-        if (tid == 0) s_last = lo;
-    }
-    __syncthreads();
-    const uint32_t m = s_last - b, share = (m + NS - 1) / NS;
-    const Cols<VEC> c(a.D, L, ln);
-    const int64_t col = c.col;
-    const bool on = c.on;
+    const int s = threadIdx.x / L, NS = 256 / L;
+    const uint32_t share = (m + NS - 1) / NS;
     float acc[VEC] = {};
-    if (on) {
+    if (c.on) {
         const uint32_t j0 = b + 1 + min(m, s * share), j1 = b + 1 + min(m, (s + 1) * share);
 #pragma unroll 8
         for (uint32_t j = j0; j < j1; ++j) {
-            const float* p = a.head + (int64_t)j * a.D + col;
+            const float* p = a.head + (int64_t)j * a.D + c.col;
 #pragma unroll
-            for (int c = 0; c < VEC; ++c) acc[c] += p[c];
+            for (int k = 0; k < VEC; ++k) acc[k] += p[k];
         }
     }
-    if (on && s == 0) {
-        const float* p = a.tail + (int64_t)b * a.D + col;
+    if (c.on && s == 0) {
+        const float* p = a.tail + (int64_t)b * a.D + c.col;
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) acc[c] += p[c];
+        for (int k = 0; k < VEC; ++k) acc[k] += p[k];
     }
     sum_subgroups<VEC>(part, acc, L, m < (uint32_t)NS ? (int)m : NS);
-    if (s == 0 && on) put_row<OT, VEC>(a, v, c, acc);
+    if (s == 0 && c.on) put_row<OT, VEC>(a, v, c, acc);
+}
+
+// One workgroup per workgroup of the sums: if a run begins in it and goes on, into at most kLong others,
+// it joins the run's sums.  Longer runs cross the start of a workgroup whose number kLong divides: for each of
+// those there are workgroups of strips of 8 lanes' columns, so that a long run's many heads are read by
+// many units (100k rows of 256 bf16 that are all one row's: 7.9 us, 35.5 by one workgroup).
+constexpr uint32_t kLong = 64;  // a wave's lanes
+constexpr int kStripLanes = 8;
+
+template <typename OT, typename I, int VEC>
+__global__ __launch_bounds__(256) void embed_join_kernel(const SumArgs<I> a, uint32_t zero_blocks) {
+    __shared__ uint32_t s_run[2];
+    const int tid = threadIdx.x, L = a.lanes, ln = tid & (L - 1), NS = 256 / L;
+    const bool asc = a.ascend && *a.ascend;
+    const uint32_t E = NS * a.run;
+    uint32_t b = blockIdx.x;
+    if (b >= a.blocks + zero_blocks) {
+        constexpr int SV = VEC < 4 ? VEC : 4;
+        const uint32_t strips = (uint32_t)((a.D + kStripLanes * SV - 1) / (kStripLanes * SV));
+        const uint32_t k = (b - a.blocks - zero_blocks) * gridDim.y + blockIdx.y, at = (k / strips + 1) * kLong;
+        if (at >= a.blocks) return;
+        const uint32_t v = sorted_id(a, asc, at * E), from = at - kLong;
+        if (v >= a.V || sorted_id(a, asc, at * E - 1) != v) return;
+        if (from && sorted_id(a, asc, from * E) == v && sorted_id(a, asc, from * E - 1) == v) return;  // an earlier one's
+        if (tid < 64) {  // the first workgroup that ends with v
+            const uint64_t ends = __ballot(sorted_id(a, asc, (from + tid + 1) * E - 1) == v);
+            const uint32_t last = last_with(a, asc, E, v, at);
+            if (tid == 0) {
+                s_run[0] = from + __ffsll((unsigned long long)ends) - 1;
+                s_run[1] = last;
+            }
+        }
+        __syncthreads();
+        b = s_run[0];
+        const uint32_t m = s_run[1] - b;
+        const Cols<SV> c(a.D, kStripLanes, tid & (kStripLanes - 1), k % strips);
+        if (m > kLong) join_run<OT, SV>(a, v, b, m, kStripLanes, c);
+        return;
+    }
+    if (b >= a.blocks) {
+        if (asc) zero_between<OT, VEC>(a, (b - a.blocks) * a.rows);
+        return;
+    }
+    const uint32_t i0 = b * E, i1 = i0 + E;
+    if (i1 >= a.n) return;
+    const uint32_t v = sorted_id(a, asc, i1), v1 = sorted_id(a, asc, i1 - 1), v0 = sorted_id(a, asc, b ? i0 - 1 : i1);
+    if (v >= a.V || v1 != v || (b && v0 == v)) return;
+    if (tid < 64) {
+        const uint32_t last = last_with(a, asc, E, v, b + 1);
+        if (tid == 0) s_run[0] = last;
+    }
+    __syncthreads();
+    const uint32_t m = s_run[0] - b;
+    if (m <= kLong) join_run<OT, VEC>(a, v, b, m, L, Cols<VEC>(a.D, L, ln, blockIdx.y));
 }
 
 // ---------------------------------------------------------------------------------- launches
@@ -1132,9 +1176,13 @@ static void launch_sums(const BwdPlan& p, const SumArgs<I>& a, uint32_t zero_blo
         default:
             hipLaunchKernelGGL((embed_sum_kernel<GT, OT, I, VEC>), dim3(a.blocks, p.slabs), block,
                                (2 * (256 / a.lanes) * a.run + 2) * sizeof(uint32_t), s, a);
-            if (a.blocks + zero_blocks > 1)
-                hipLaunchKernelGGL((embed_join_kernel<OT, I, VEC>), dim3(a.blocks + zero_blocks, p.slabs), block, 0, s,
-                                   a);
+            if (a.blocks + zero_blocks > 1) {
+                constexpr int strip = kStripLanes * (VEC < 4 ? VEC : 4);
+                const uint64_t strips = (uint64_t)((a.D + strip - 1) / strip) * ((a.blocks - 1) / kLong);
+                const uint32_t longs = (uint32_t)((strips + p.slabs - 1) / p.slabs);
+                hipLaunchKernelGGL((embed_join_kernel<OT, I, VEC>), dim3(a.blocks + zero_blocks + longs, p.slabs), block, 0,
+                                   s, a, zero_blocks);
+            }
     }
 }
 
@@ -1164,8 +1212,9 @@ static int launch_bwd(const BwdPlan& p, char* w, SumArgs<I> a, const void* ids, 
     uint32_t zero_blocks = 0;
     const size_t dw_bytes = (size_t)a.V * a.D * elem_size(dwtype);
     if ((p.form == kFew || p.form == kRadix) && !a.accumulate) {  // about 32 KB of zeros per workgroup
-        const int64_t rows = 32768 / ((int64_t)p.lanes * vec * elem_size(dwtype));
-        a.rows = (uint32_t)(rows < 1 ? 1 : rows > kFewRows ? kFewRows : rows);
+        int64_t rows = 32768 / ((int64_t)p.lanes * vec * elem_size(dwtype));
+        while (a.V / rows > 1 << 23) rows *= 2;  // a launch holds fewer than 2^24 workgroups
+        a.rows = (uint32_t)(rows > kFewRows ? kFewRows : rows);
         zero_blocks = (a.V + a.rows - 1) / a.rows;
     }
     if (p.form == kBucket || p.form == kRadix)
@@ -1301,7 +1350,7 @@ extern "C" int hgsr_embed_bwd(int64_t V, int64_t n, int64_t D, const void* g, in
         set_error("embed_bwd: workspace of %zu bytes, %zu needed", ws ? ws_bytes : (size_t)0, p.bytes);
         return HGSR_EWORKSPACE;
     }
-    HGSR_REQUIRE(p.blocks < (1u << 24), "embed_bwd: %lld ids of rows of %lld: too many for a launch", (long long)n,
+    HGSR_REQUIRE(p.blocks <= (1u << 22), "embed_bwd: %lld ids of rows of %lld: too many for a launch", (long long)n,
                  (long long)D);
     char* w = static_cast<char*>(ws);
     auto run = [&](auto none) {

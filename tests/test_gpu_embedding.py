@@ -145,6 +145,28 @@ def test_grad_of_whole_numbers_is_exact(V, n, D, kind):
     assert torch.equal(out.double(), want.double() + 1)
 
 
+@pytest.mark.parametrize("D,near", [(257, 4096), (33, 32_768), (2, 65_536), (600, 64)])
+@pytest.mark.parametrize("order", ["sorted", "shuffled"])
+def test_runs_of_many_lengths_are_exact(D, near, order):
+    """Rows that about `near` ids name (what a hundred workgroups' worth of entries comes to, and one), some
+    exactly as many, with rows of one or a few ids between them."""
+    g0 = gen(D + near)
+    length = torch.randint(near - near // 8, near + near // 8 + 1, (9,), generator=g0).tolist()
+    length = [1, near, near + 1, 3, 2 * near, *length[:5], 1, 2, near - 1, *length[5:], 3 * near]
+    V = 3 * len(length) + 1
+    ids = torch.repeat_interleave(3 * torch.arange(len(length)) + 1, torch.tensor(length))
+    if order == "shuffled":
+        ids = ids[torch.randperm(ids.numel(), generator=g0)]
+    ids = ids.to(DEV)
+    for t in (F32, BF16):
+        g = torch.randint(-8, 9, (ids.numel(), D), generator=g0).to(DEV)
+        want = torch.zeros(V, D, dtype=torch.int64, device=DEV).index_add_(0, ids, g)
+        assert torch.equal(E.embedding_grad(g.to(t), ids, V, dtype=F32).double(), want.double())
+        out = torch.ones(V, D + 1, device=DEV)
+        E.embedding_grad(g.to(t), ids, V, out=out[:, 1:])
+        assert torch.equal(out[:, 1:].double(), want.double() + 1) and out[:, 0].eq(1).all()
+
+
 def test_strides_and_shapes():
     g0 = gen(1)
     wide = torch.randn(50, 45, generator=g0)
