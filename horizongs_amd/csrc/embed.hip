@@ -699,8 +699,12 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const SumArgs<I> a) {
 
 // ---- few rows: no sort.  Every subgroup keeps a table of sums in LDS, its own, so a workgroup's
 // entries are read once and in order; the subgroups' and then the workgroups' tables are added.
-// 500k ids of rows of 32 floats: 16 rows 20.8 us (sorted: 37.8), 32 rows 25.2 (sorted: 37.6).
+// 500k ids of rows of 32 floats: 16 rows 20.0 us (sorted: 37.8), 32 rows 24.0 (sorted: 37.6).
 constexpr int kTableMost = 128;  // V * VEC: 128 KB of LDS
+// Rows that a subgroup reads at once: the tables leave room for one or two workgroups per unit, so each has
+// to keep many loads in flight.  500k ids, 20 rows of 64 floats: 8 / 12 / 16 / 24 rows 52 / 44 / 43 / 52 us;
+// 16 rows of 16 bf16: 24 / 19 / 18.7 / 24.
+constexpr int kTableRounds = 16;
 
 template <typename GT, typename I, int VEC>
 __global__ __launch_bounds__(256) void embed_table_kernel(const SumArgs<I> a) {
@@ -719,11 +723,11 @@ __global__ __launch_bounds__(256) void embed_table_kernel(const SumArgs<I> a) {
     __syncthreads();
     const GT* g = static_cast<const GT*>(a.g) + col;
     const uint64_t i1 = min((uint64_t)a.n, ((uint64_t)blockIdx.x + 1) * a.rows);
-    for (uint64_t i0 = (uint64_t)blockIdx.x * a.rows + s; i0 < i1; i0 += 8 * NS) {
-        uint32_t id[8];
-        Vec<GT, VEC> x[8];
+    for (uint64_t i0 = (uint64_t)blockIdx.x * a.rows + s; i0 < i1; i0 += kTableRounds * NS) {
+        uint32_t id[kTableRounds];
+        Vec<GT, VEC> x[kTableRounds];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
+        for (int u = 0; u < kTableRounds; ++u) {
             const int64_t i = i0 + u * NS;
             const int64_t j = i < (int64_t)i1 ? i : i1 - 1;
             id[u] = a.ids.get(j, a.V);
@@ -731,7 +735,7 @@ __global__ __launch_bounds__(256) void embed_table_kernel(const SumArgs<I> a) {
             x[u] = load_vec<GT, VEC>(g + j * a.gstride);
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < kTableRounds; ++u)
             if (id[u] < a.V) {
                 Vec<float, VEC> t = tab[id[u] * 256 + tid];
                 add_vec<GT, VEC>(t.v, x[u]);
@@ -1053,7 +1057,7 @@ static BwdPlan bwd_plan(int64_t V, int64_t n, int64_t D, int vec) {
     if (p.form == kTable) {
         int64_t blocks = (V * vec > 64 ? 256 : 512) / p.slabs;  // as many as the tables leave room for
         if (blocks < 1) blocks = 1;
-        const int64_t step = 8 * NS, rows = (n + blocks - 1) / blocks;
+        const int64_t step = kTableRounds * NS, rows = (n + blocks - 1) / blocks;
         p.rows = (uint32_t)((rows + step - 1) / step * step);
         p.blocks = (uint32_t)((n + p.rows - 1) / p.rows);
         p.head = take((size_t)p.blocks * V * D * 4);
