@@ -8,12 +8,13 @@
 Tables and rows may be float32, float16 or bfloat16; sums are f32, rounded once.  An id outside
 [0, num_rows) (-1 by custom) is padding: its row is zeros and it takes no part in the gradient --
 there is no host read that could raise.  Gradients are summed in an order that the ids, the sizes
-and the types set, so they are the same bits on every run, wherever the tensors lie.  There is no
-CPU path.
+and the types set, so they are the same bits on every run, wherever the tensors lie.  Forward-mode
+derivatives are refused.  There is no CPU path.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 from . import gradbuf
@@ -76,6 +77,12 @@ def id_stride(flat):
     return flat.stride(0) if flat.shape[0] > 1 else 1
 
 
+def _recorded(t):
+    """Whether a call on t has to go through its Function: for a gradient, or for a tangent (a dual tensor's
+    primal may need no gradient, and torch.no_grad() does not switch tangents off), which a Function refuses."""
+    return (t.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0
+
+
 def _lookup(weight, flat, shape, scale, dtype, index):
     V, D = weight.shape
     out = weight.new_empty((*shape, D), dtype=dtype)
@@ -111,7 +118,8 @@ class _Embedding(torch.autograd.Function):
     def backward(ctx, g):
         flat, = ctx.saved_tensors
         shape, dtype, key, scale, index = ctx.args
-        if torch.is_grad_enabled():  # create_graph: the gradient is linear in g, and its own gradient a lookup
+        # create_graph: the gradient is linear in g, and its own gradient a lookup
+        if torch.is_grad_enabled() or _recorded(g):
             return _EmbeddingGrad.apply(g, flat, shape, dtype, scale, index), None, None, None, None, None
         out = gradbuf.take(key, shape, dtype)  # in place in a DDP bucket when one is registered
         if out is None:
@@ -131,7 +139,7 @@ class _EmbeddingGrad(torch.autograd.Function):
         (flat,) = ctx.saved_tensors
         shape, dtype, scale, index = ctx.args
         gg = rows_view(gg, gg.shape[1], "the gradient's gradient")
-        if torch.is_grad_enabled():
+        if torch.is_grad_enabled() or _recorded(gg):
             return _Embedding.apply(gg, flat, shape[:-1], scale, dtype, index), None, None, None, None, None
         return _lookup(gg, flat, shape[:-1], scale, dtype, index), None, None, None, None, None
 
@@ -151,7 +159,7 @@ def embedding(weight, ids, scale=1.0, dtype=None):
     check_ids(ids)
     index = check_device(weight, ids)
     flat = flat_ids(ids)
-    if weight.requires_grad and torch.is_grad_enabled():
+    if _recorded(weight):
         return _Embedding.apply(weight, flat, ids.shape, float(scale), dtype, index)
     return _lookup(weight, flat, ids.shape, float(scale), dtype, index)
 
@@ -175,7 +183,7 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
         dtype = grad.dtype if dtype is None else dtype
         type_code(dtype)
         index = check_device(grad, ids)
-        if D and grad.requires_grad and torch.is_grad_enabled():
+        if D and _recorded(grad):
             return _EmbeddingGrad.apply(grad, flat_ids(ids), (num_rows, D), dtype, float(scale), index)
         out, accumulate = grad.new_empty((num_rows, D), dtype=dtype), 0
     else:
@@ -187,6 +195,8 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
             raise ValueError("hgsr: the rows of out overlap")
         if torch.is_grad_enabled() and (grad.requires_grad or out.requires_grad):
             raise NotImplementedError("hgsr: sums added to out are not differentiable (torch.no_grad())")
+        if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (grad, out)):
+            raise NotImplementedError("hgsr: sums added to out are not differentiable, in forward mode neither")
         index, accumulate = check_device(grad, ids, out), 1
     g = rows_view(grad, D, "grad") if D else grad
     return _grad(g, flat_ids(ids), out, float(scale), accumulate, index)

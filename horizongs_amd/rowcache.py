@@ -11,7 +11,7 @@ s = max(max |x| over the group * (1 / 127) (e4m3: 1 / 448), 2^-100) in f32 and x
 code, ties to even; x' = code * s reads back within s / 2 (int8), or within 2^-4 of each value and 2^-10 s (e4m3).  A
 group that holds a NaN or an infinity reads back as NaN.  decode.decode() takes a cache for the anchor
 features: the visible anchors' rows are read back for each view (a quarter of their float32 bytes are
-kept, plus the scales).  No gradient passes through a cache.  There is no CPU path.
+kept, plus the scales).  No derivative passes through a cache, in reverse or in forward mode.  There is no CPU path.
 """
 from __future__ import annotations
 

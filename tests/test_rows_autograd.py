@@ -1,0 +1,78 @@
+"""CPU tests of what autograd sees of the row tables' calls (horizongs_amd.embedding, horizongs_amd.rowcache).
+
+The native entries are replaced by their formulas on host memory (contiguous float32 rows, int64 numbers);
+what is tested is the Python boundary around them."""
+import ctypes as ct
+
+import numpy as np
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from horizongs_amd import _native as N
+from horizongs_amd import embedding as E
+from horizongs_amd import rowcache as R
+
+
+def at(ptr, ctype, *shape):
+    return np.ctypeslib.as_array(ct.cast(ptr, ct.POINTER(ctype)), shape)
+
+
+def formulas(index, name, *a):
+    if name == "hgsr_embed_fwd":
+        V, n, D, w, _, _, ids, _, _, scale, out, _ = a
+        at(out, ct.c_float, n, D)[:] = at(w, ct.c_float, V, D)[at(ids, ct.c_int64, n)] * scale
+    elif name == "hgsr_embed_bwd":
+        V, n, D, g, _, _, ids, _, _, scale, dw, _, _, accumulate, _, _ = a
+        if not accumulate:
+            at(dw, ct.c_float, V, D)[:] = 0
+        np.add.at(at(dw, ct.c_float, V, D), at(ids, ct.c_int64, n), at(g, ct.c_float, n, D) * scale)
+    elif name == "hgsr_rowcache_write":  # codes: the slot's last row rounded, scales 1
+        cap, n, D, group, _, x, _, _, slots, _, _, codes, _, scales, _, _, _ = a
+        at(codes, ct.c_int8, cap, D)[at(slots, ct.c_int64, n)] = np.rint(at(x, ct.c_float, n, D))
+        at(scales, ct.c_float, cap, -(-D // group))[at(slots, ct.c_int64, n)] = 1
+    else:
+        assert name == "hgsr_rowcache_read"
+        cap, n, D, group, _, codes, _, scales, _, slots, _, _, out, _ = a
+        k = at(slots, ct.c_int64, n)
+        at(out, ct.c_float, n, D)[:] = at(codes, ct.c_int8, cap, D)[k] * at(scales, ct.c_float, cap, -(-D // group))[k][:, :1]
+
+
+@pytest.fixture(autouse=True)
+def on_the_host(monkeypatch):
+    monkeypatch.setattr(N, "call_on", formulas)
+    monkeypatch.setattr(N, "size_query", lambda *a: 0)
+    for m in (E, R):
+        monkeypatch.setattr(m, "check_device", lambda *ts: 0)
+
+
+IDS = torch.tensor([2, 0, 2])
+
+
+def table(V=4, D=3):
+    return torch.arange(float(V * D)).reshape(V, D)
+
+
+def test_forward_mode_is_refused_not_dropped():
+    """A dual tensor's primal needs no gradient; its tangent must not get lost on the way."""
+    w, g = table(), torch.ones(3, 3)
+    with forward_ad.dual_level():
+        dw, dg = forward_ad.make_dual(w, torch.ones_like(w)), forward_ad.make_dual(g, torch.ones_like(g))
+        for call in (lambda: E.embedding(dw, IDS, 2.0), lambda: E.embedding_grad(dg, IDS, 4),
+                     lambda: E.embedding_grad(dg, IDS, 4, out=table()), lambda: E.embedding_grad(g, IDS, 4, out=dw)):
+            with pytest.raises(NotImplementedError, match="jvp|forward mode"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="jvp|forward mode"):
+                call()
+        # a backward pass along a dual gradient
+        p = table().requires_grad_(True)
+        with pytest.raises(NotImplementedError, match="jvp"):
+            torch.autograd.grad(E.embedding(p, IDS), p, dg)
+        q = g.clone().requires_grad_(True)
+        with pytest.raises(NotImplementedError, match="jvp"):
+            torch.autograd.grad(E.embedding_grad(q, IDS, 4), q, dw)
+        # tensors without a tangent, at the same level
+        assert torch.equal(E.embedding(w, IDS, 2.0), 2 * w[IDS])
+        out = E.embedding_grad(g, IDS, 4, out=table())
+        assert torch.equal(E.embedding_grad(g, IDS, 4) + w, out)
+    assert torch.equal(E.embedding(w, IDS, 2.0), 2 * w[IDS])
