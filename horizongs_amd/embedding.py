@@ -9,7 +9,7 @@ Tables and rows may be float32, float16 or bfloat16; sums are f32, rounded once.
 [0, num_rows) (-1 by custom) is padding: its row is zeros and it takes no part in the gradient --
 there is no host read that could raise.  Gradients are summed in an order that the ids, the sizes
 and the types set, so they are the same bits on every run, wherever the tensors lie.  Forward-mode
-derivatives are refused.  There is no CPU path.
+derivatives and torch.jit.trace are refused.  There is no CPU path.
 """
 from __future__ import annotations
 
@@ -75,6 +75,12 @@ def flat_ids(ids):
 
 def id_stride(flat):
     return flat.stride(0) if flat.shape[0] > 1 else 1
+
+
+def refuse_trace():
+    """torch.jit.trace would record the allocation of a result and not the call that fills it."""
+    if torch._C._get_tracing_state() is not None:
+        raise NotImplementedError("hgsr: calls on row tables cannot be traced")
 
 
 def _recorded(t):
@@ -148,6 +154,7 @@ def embedding(weight, ids, scale=1.0, dtype=None):
     """scale * weight[ids]: weight [V, D] (any row stride, contiguous columns), ids int32 / int64 of
     any shape; returns [*ids.shape, D] in `dtype` (default: weight's).  The product is f32, rounded
     once.  Differentiable in weight; the gradient has weight's type and a row for each of its rows."""
+    refuse_trace()
     if weight.dim() != 2:
         raise ValueError(f"hgsr: weight must be [rows, columns], not {tuple(weight.shape)}")
     type_code(weight.dtype)
@@ -172,6 +179,7 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
     to its named rows instead -- each row's sum and its old value are added in f32 and rounded once,
     the other rows are left as they are -- and out, which must not share memory with grad, is
     returned; nothing is differentiated through that."""
+    refuse_trace()
     type_code(grad.dtype)
     check_ids(ids)
     if grad.dim() < 1 or grad.shape[:-1] != ids.shape:

@@ -11,7 +11,8 @@ s = max(max |x| over the group * (1 / 127) (e4m3: 1 / 448), 2^-100) in f32 and x
 code, ties to even; x' = code * s reads back within s / 2 (int8), or within 2^-4 of each value and 2^-10 s (e4m3).  A
 group that holds a NaN or an infinity reads back as NaN.  decode.decode() takes a cache for the anchor
 features: the visible anchors' rows are read back for each view (a quarter of their float32 bytes are
-kept, plus the scales).  No derivative passes through a cache, in reverse or in forward mode.  There is no CPU path.
+kept, plus the scales).  No derivative passes through a cache, in reverse or in forward mode, and
+its calls cannot be traced.  There is no CPU path.
 """
 from __future__ import annotations
 
@@ -20,7 +21,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native as N
-from .embedding import _TYPES, check_device, check_ids, id_stride, row_stride, type_code
+from .embedding import _TYPES, check_device, check_ids, id_stride, refuse_trace, row_stride, type_code
 
 _FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _NAMES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
@@ -46,6 +47,7 @@ def rowcache_alloc(capacity, dim, fmt="int8", group=32, device="cuda"):
 
 
 def _cache(cache):
+    refuse_trace()
     codes, scales, group = cache
     if group not in GROUPS:
         raise ValueError(f"hgsr row cache: group of {group} columns: one of {GROUPS}")

@@ -76,3 +76,17 @@ def test_forward_mode_is_refused_not_dropped():
         out = E.embedding_grad(g, IDS, 4, out=table())
         assert torch.equal(E.embedding_grad(g, IDS, 4) + w, out)
     assert torch.equal(E.embedding(w, IDS, 2.0), 2 * w[IDS])
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("grad", [False, True])
+def test_traces_are_refused(grad):
+    """A trace would hold the new tensor and not the call that fills it."""
+    w, g = table().requires_grad_(grad), torch.ones(3, 3, requires_grad=grad)
+    c, t = R.rowcache_alloc(4, 3, device="cpu"), table()
+    for call in (lambda w, g, i: E.embedding(w, i), lambda w, g, i: E.embedding_grad(g, i, 4),
+                 lambda w, g, i: E.embedding_grad(g.detach(), i, 4, out=t), lambda w, g, i: R.rowcache_read(c, i),
+                 lambda w, g, i: (R.rowcache_write(c, g, i), g)[1]):
+        with pytest.raises(NotImplementedError, match="traced"):
+            torch.jit.trace(call, (w, g, IDS), check_trace=False)
+    assert not c.scales.any() and torch.equal(t, table())
