@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _native as N
 from . import gradbuf
@@ -207,7 +208,10 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
             raise NotImplementedError("hgsr: sums added to out are not differentiable, in forward mode neither")
         index, accumulate = check_device(grad, ids, out), 1
     g = rows_view(grad, D, "grad") if D else grad
-    return _grad(g, flat_ids(ids), out, float(scale), accumulate, index)
+    _grad(g, flat_ids(ids), out, float(scale), accumulate, index)
+    if accumulate and grad.numel():
+        increment_version(out)  # a backward that saved out as it was must not go on with it
+    return out
 
 
 class Embedding(torch.nn.Module):

@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _native as N
 from .embedding import _TYPES, check_device, check_ids, id_stride, refuse_trace, row_stride, type_code
@@ -100,6 +101,7 @@ def rowcache_write(cache, rows, slots=None):
     ws = torch.empty(ws_b, dtype=torch.uint8, device=codes.device) if ws_b else None
     N.call_on(index, "hgsr_rowcache_write", capacity, n, dim, group, _FORMATS[codes.dtype], rows.data_ptr(), xt, xs,
               *_slot_args(slots), codes.data_ptr(), cs, scales.data_ptr(), ss, ws.data_ptr() if ws_b else None, ws_b)
+    increment_version((codes, scales))  # a backward that saved them as they were must not go on with them
 
 
 def rowcache_read(cache, slots=None, dtype=torch.float32):

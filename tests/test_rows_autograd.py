@@ -90,3 +90,45 @@ def test_traces_are_refused(grad):
         with pytest.raises(NotImplementedError, match="traced"):
             torch.jit.trace(call, (w, g, IDS), check_trace=False)
     assert not c.scales.any() and torch.equal(t, table())
+
+
+def test_sums_added_to_a_saved_table_are_seen():
+    """A backward pass that saved the table as it was refuses to go on with the changed one."""
+    for view in (lambda t: t, lambda t: t[1:3]):
+        base = table(6, 3)
+        p = torch.ones_like(base, requires_grad=True)
+        y = (p * base).sum()
+        E.embedding_grad(torch.empty(0, 3), IDS[:0], view(base).shape[0], out=view(base))
+        assert base._version == 0  # no rows: nothing was added
+        t = view(base)
+        E.embedding_grad(torch.ones(2, 3), torch.tensor([1, 1]), t.shape[0], out=t)
+        assert t._version == base._version == 1
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    with torch.inference_mode():
+        t = table()
+        E.embedding_grad(torch.ones(3, 3), IDS, 4, out=t)
+    E.embedding_grad(torch.ones(3, 3), IDS, 4, out=t)  # an inference tensor has no version
+    assert float(t[2, 0]) == 6 + 4
+    leaf = table().requires_grad_(True)  # the documented way to a leaf
+    y = leaf.square().sum()
+    with torch.no_grad():
+        E.embedding_grad(torch.ones(3, 3), IDS, 4, out=leaf)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+
+
+def test_writes_to_a_saved_cache_are_seen():
+    c = R.rowcache_alloc(4, 3, device="cpu")
+    p = torch.ones(4, 1, requires_grad=True)
+    before = c.codes._version, c.scales._version
+    R.rowcache_write(c, torch.empty(0, 3), IDS[:0])
+    assert (c.codes._version, c.scales._version) == before
+    for saved in (c.scales, c.codes):
+        y = (p * saved).sum()
+        R.rowcache_write(c, torch.ones(3, 3), IDS)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    before = c.codes._version, c.scales._version
+    assert torch.equal(R.rowcache_read(c, IDS), torch.ones(3, 3))
+    assert (c.codes._version, c.scales._version) == before
