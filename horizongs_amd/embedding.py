@@ -58,7 +58,7 @@ def rows_view(t, dim, what):
     if t.shape[-1] != dim:
         raise ValueError(f"hgsr: rows of {what} have {t.shape[-1]} columns, not {dim}")
     if t.dim() != 2:
-        t = t.reshape(-1, dim)
+        t = t.reshape(t.shape[:-1].numel(), dim)  # spelt out: rows may have no columns
     return t if dim == 1 or t.stride(1) == 1 else t.contiguous()
 
 
@@ -192,7 +192,7 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
         dtype = grad.dtype if dtype is None else dtype
         type_code(dtype)
         index = check_device(grad, ids)
-        if D and _recorded(grad):
+        if _recorded(grad):
             return _EmbeddingGrad.apply(grad, flat_ids(ids), (num_rows, D), dtype, float(scale), index)
         out, accumulate = grad.new_empty((num_rows, D), dtype=dtype), 0
     else:
@@ -207,8 +207,7 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
         if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (grad, out)):
             raise NotImplementedError("hgsr: sums added to out are not differentiable, in forward mode neither")
         index, accumulate = check_device(grad, ids, out), 1
-    g = rows_view(grad, D, "grad") if D else grad
-    _grad(g, flat_ids(ids), out, float(scale), accumulate, index)
+    _grad(rows_view(grad, D, "grad"), flat_ids(ids), out, float(scale), accumulate, index)
     if accumulate and grad.numel():
         increment_version(out)  # a backward that saved out as it was must not go on with it
     return out

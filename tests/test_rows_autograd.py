@@ -15,6 +15,8 @@ from horizongs_amd import rowcache as R
 
 
 def at(ptr, ctype, *shape):
+    if not all(shape):
+        return np.empty(shape, ctype)  # such tensors have no memory
     return np.ctypeslib.as_array(ct.cast(ptr, ct.POINTER(ctype)), shape)
 
 
@@ -132,3 +134,27 @@ def test_writes_to_a_saved_cache_are_seen():
     before = c.codes._version, c.scales._version
     assert torch.equal(R.rowcache_read(c, IDS), torch.ones(3, 3))
     assert (c.codes._version, c.scales._version) == before
+
+
+@pytest.mark.parametrize("shape", [(), (3,), (2, 3), (0,), (2, 0), (0, 2)])
+@pytest.mark.parametrize("D", [0, 1, 3])
+def test_gradients_of_every_shape(shape, D):
+    """Tables without columns, no ids, ids of any number of dimensions: forward, backward, second derivative."""
+    V = 4
+    ids = torch.randint(0, V, shape)
+    w = torch.randn(V, D, requires_grad=True)
+    y = E.embedding(w, ids, 2.0)
+    assert y.shape == (*shape, D)
+    g = torch.randn(*shape, D)
+    (dw,) = torch.autograd.grad(y, w, g)
+    v = w.detach().clone().requires_grad_(True)
+    (want,) = torch.autograd.grad(2.0 * v[ids], v, g)
+    assert torch.allclose(dw, want) and dw.shape == (V, D)
+    assert torch.equal(E.embedding_grad(g, ids, V, 2.0), dw)
+    assert torch.equal(E.embedding_grad(g, ids, V, 2.0, out=torch.zeros(V, D)), dw)
+    q = g.clone().requires_grad_(True)
+    (dq,) = torch.autograd.grad(E.embedding_grad(q, ids, V, 2.0), q, w.detach())
+    assert torch.equal(dq, y.detach())
+    (x,) = torch.autograd.grad(E.embedding(w, ids).square().sum(), w, create_graph=True)
+    (xx,) = torch.autograd.grad(x, w, torch.ones_like(w))
+    assert torch.allclose(xx, 2.0 * torch.bincount(ids.reshape(-1), minlength=V)[:, None].expand(V, D).float())
