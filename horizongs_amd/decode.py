@@ -281,7 +281,7 @@ def _decode_cached(anchor, feat, offset, scaling_raw, vis_idx):
         vi = vis_idx
         vis_idx = vi.buf[:int(vi.counts[1].item())]  # the compacted arrays need their length on the host
         _VIS_CACHE[:] = [(vi.visible, vi.visible._version, vis_idx)]
-    take = lambda t: embedding(_f32(t).reshape(t.shape[0], -1), vis_idx).reshape(-1, *t.shape[1:])
+    take = lambda t: embedding(_f32(t).flatten(1), vis_idx).reshape(-1, *t.shape[1:])
     return take(anchor), rowcache_read(feat, vis_idx), take(offset), take(scaling_raw)
 
 

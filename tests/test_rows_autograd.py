@@ -1,51 +1,19 @@
 """CPU tests of what autograd sees of the row tables' calls (horizongs_amd.embedding, horizongs_amd.rowcache).
 
-The native entries are replaced by their formulas on host memory (contiguous float32 rows, int64 numbers);
-what is tested is the Python boundary around them."""
-import ctypes as ct
-
-import numpy as np
+The native entries are replaced by their formulas on host memory; what is tested is the Python boundary
+around them."""
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from horizongs_amd import _native as N
 from horizongs_amd import embedding as E
 from horizongs_amd import rowcache as R
-
-
-def at(ptr, ctype, *shape):
-    if not all(shape):
-        return np.empty(shape, ctype)  # such tensors have no memory
-    return np.ctypeslib.as_array(ct.cast(ptr, ct.POINTER(ctype)), shape)
-
-
-def formulas(index, name, *a):
-    if name == "hgsr_embed_fwd":
-        V, n, D, w, _, _, ids, _, _, scale, out, _ = a
-        at(out, ct.c_float, n, D)[:] = at(w, ct.c_float, V, D)[at(ids, ct.c_int64, n)] * scale
-    elif name == "hgsr_embed_bwd":
-        V, n, D, g, _, _, ids, _, _, scale, dw, _, _, accumulate, _, _ = a
-        if not accumulate:
-            at(dw, ct.c_float, V, D)[:] = 0
-        np.add.at(at(dw, ct.c_float, V, D), at(ids, ct.c_int64, n), at(g, ct.c_float, n, D) * scale)
-    elif name == "hgsr_rowcache_write":  # codes: the slot's last row rounded, scales 1
-        cap, n, D, group, _, x, _, _, slots, _, _, codes, _, scales, _, _, _ = a
-        at(codes, ct.c_int8, cap, D)[at(slots, ct.c_int64, n)] = np.rint(at(x, ct.c_float, n, D))
-        at(scales, ct.c_float, cap, -(-D // group))[at(slots, ct.c_int64, n)] = 1
-    else:
-        assert name == "hgsr_rowcache_read"
-        cap, n, D, group, _, codes, _, scales, _, slots, _, _, out, _ = a
-        k = at(slots, ct.c_int64, n)
-        at(out, ct.c_float, n, D)[:] = at(codes, ct.c_int8, cap, D)[k] * at(scales, ct.c_float, cap, -(-D // group))[k][:, :1]
+from tests import rows_on_host
 
 
 @pytest.fixture(autouse=True)
 def on_the_host(monkeypatch):
-    monkeypatch.setattr(N, "call_on", formulas)
-    monkeypatch.setattr(N, "size_query", lambda *a: 0)
-    for m in (E, R):
-        monkeypatch.setattr(m, "check_device", lambda *ts: 0)
+    rows_on_host.install(monkeypatch)
 
 
 IDS = torch.tensor([2, 0, 2])
