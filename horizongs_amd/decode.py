@@ -329,8 +329,12 @@ def decode(anchor, feat, offset, scaling_raw, cam_center, mlps, visible=None, vi
             from .rowcache import rowcache_read
             feat = rowcache_read(feat)
         else:
-            idx = visible if isinstance(visible, VisibleIndex) else visible_index(visible) \
-                if visible.dtype == torch.bool else visible.reshape(-1)
+            if isinstance(visible, VisibleIndex):
+                idx = visible
+            elif visible.dtype == torch.bool:
+                idx = visible_index(visible)
+            else:
+                idx = visible.reshape(-1).to(torch.int32)  # of any integer type, as below
             anchor, feat, offset, scaling_raw = _decode_cached(anchor, feat, offset, scaling_raw, idx)
             visible, A = None, anchor.shape[0]
     if visible is None:

@@ -56,3 +56,26 @@ def test_a_cache_of_an_empty_model(calls, visible):
     t, w, cache = scene(0)
     decode(t, cache, w, visible)
     assert [tuple(x.shape) for x in compacted(calls)] == [(0, 3), (0, F), (0, N_OFF, 3), (0, 6)]
+
+
+@pytest.mark.parametrize("kind", [torch.uint8, torch.int16, torch.int32, torch.int64, torch.bool, None, "lazy"])
+def test_indices_of_a_cached_decode(calls, kind):
+    """Every kind of index that a decode of float32 features takes."""
+    t, w, cache = scene(40)
+    idx = torch.tensor([3, 4, 9, 17, 39])
+    if kind == torch.bool:
+        visible = torch.zeros(40, dtype=kind)
+        visible[idx] = True
+    elif kind == "lazy":
+        buf = torch.full((40,), -7, dtype=torch.int32)
+        buf[:5] = idx
+        visible = HD.VisibleIndex(buf, torch.tensor([0, 5]), torch.ones(40, dtype=torch.bool))
+    else:
+        visible, idx = (None, torch.arange(40)) if kind is None else (idx.to(kind), idx)
+    decode(t, cache, w, visible)
+    got = compacted(calls)
+    for x, k in zip(got, ("anchor", "feat", "offset", "scaling")):
+        assert torch.equal(x, t[k][idx])
+    if kind != "lazy":
+        decode(t, t["feat"], w, visible)
+        assert all(torch.equal(x, y) for x, y in zip(got, compacted(calls)))
