@@ -334,7 +334,9 @@ def decode(anchor, feat, offset, scaling_raw, cam_center, mlps, visible=None, vi
             elif visible.dtype == torch.bool:
                 idx = visible_index(visible)
             else:
-                idx = visible.reshape(-1).to(torch.int32)  # of any integer type, as below
+                idx = visible.reshape(-1)
+                if idx.dtype not in (torch.int32, torch.int64):
+                    idx = idx.to(torch.int32)
             anchor, feat, offset, scaling_raw = _decode_cached(anchor, feat, offset, scaling_raw, idx)
             visible, A = None, anchor.shape[0]
     if visible is None:
