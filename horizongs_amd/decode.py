@@ -310,15 +310,17 @@ def decode(anchor, feat, offset, scaling_raw, cam_center, mlps, visible=None, vi
                 raise NotImplementedError("hgsr decode: MLPs must be Linear -> ReLU -> Linear [-> Tanh]")
             weights += [m[0].weight, m[0].bias, m[2].weight, m[2].bias]
     A = anchor.shape[0]
+    # inputs of the opacity and the colour head's first layers (a dict's weights may be flattened)
+    n_in, n_color = (weights[i].numel() // max(weights[i + 1].numel(), 1) for i in (0, 8))
     if appearance is not None:
-        w1, b1 = weights[8:10]
-        k = w1.shape[1] - appearance.numel()
+        w1, b1 = weights[8].reshape(weights[9].numel(), n_color), weights[9]
+        k = n_color - appearance.numel()
         _check_dev(appearance)
-        if k != weights[0].shape[1]:
+        if k != n_in:
             raise ValueError(f"hgsr decode: an appearance row of {appearance.numel()} does not fit the colour head's "
-                             f"{w1.shape[1]} inputs")
+                             f"{n_color} inputs")
         weights[8:10] = w1[:, :k], b1 + (w1[:, k:] * appearance.reshape(1, -1)).sum(1)
-    elif weights[8].shape[1] != weights[0].shape[1]:
+    elif n_color != n_in:
         raise ValueError("hgsr decode: the colour head takes an appearance row, and none is given")
     if cached:
         if feat[0].shape[0] != A:

@@ -79,3 +79,21 @@ def test_indices_of_a_cached_decode(calls, kind):
     if kind != "lazy":
         decode(t, t["feat"], w, visible)
         assert all(torch.equal(x, y) for x, y in zip(got, compacted(calls)))
+
+
+def test_flattened_weights(calls):
+    """A dict's weights are read by their memory, whatever their shape; with a row, too."""
+    t, w, cache = scene(7)
+    flat = {k: v.reshape(-1) for k, v in w.items()}
+    decode(t, t["feat"], flat, None)
+    assert all(x is y for x, y in zip(calls[7:], flat.values()))
+    row = torch.randn(5)
+    first = torch.randn(F, K + 5)
+    for a, b in ((first, w), (first.reshape(-1), flat)):
+        decode(t, t["feat"], dict(b, color_w1=a), None, appearance=row)
+        assert torch.equal(calls[7 + 8], first[:, :K])
+        assert torch.allclose(calls[7 + 9], w["color_b1"] + first[:, K:] @ row, atol=1e-5)
+        with pytest.raises(ValueError, match="appearance row"):
+            decode(t, t["feat"], dict(b, color_w1=a), None)
+        with pytest.raises(ValueError, match="does not fit"):
+            decode(t, t["feat"], dict(b, color_w1=a), None, appearance=row[:4])
