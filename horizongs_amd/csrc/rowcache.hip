@@ -135,7 +135,10 @@ static bool few_slots(int64_t n, int64_t D) { return n <= kFewSlots && n * n * D
 // LDS first (270k rows of 12 into 404: 16 us, 105 by atomics).
 constexpr int kSlotTile = 1024;
 constexpr int kFewCapacity = 16384;
-constexpr int kSlotWide = 16384;  // rows per workgroup of the LDS form
+constexpr int kSlotWide = 16384;  // rows per workgroup and turn of the LDS form
+// Every workgroup of the second launch reads all tiles' verdicts, so its grid does not grow with the rows: at
+// most kSlotTile workgroups read no more verdicts than there are rows.
+constexpr uint32_t kSlotBlocks = kSlotTile, kSlotWideBlocks = 256;
 
 struct SlotWork {
     uint32_t* distinct;  // [1 + tiles]: the verdict, then the tiles' own
@@ -182,14 +185,18 @@ __global__ __launch_bounds__(1024) void slot_last_few_kernel(uint32_t n, RowIds<
     __shared__ int32_t last[kFewCapacity];
     if (slots_distinct(w)) return;
     for (uint32_t s = threadIdx.x; s < capacity; s += 1024) last[s] = -1;
-    const uint32_t i0 = blockIdx.x * kSlotWide + threadIdx.x;
-    uint32_t c[kSlotWide / 1024];
+    for (uint32_t base = blockIdx.x * kSlotWide;; base += gridDim.x * kSlotWide) {
+        const uint32_t i0 = base + threadIdx.x;
+        uint32_t c[kSlotWide / 1024];
 #pragma unroll
-    for (int k = 0; k < kSlotWide / 1024; ++k) c[k] = i0 + k * 1024 < n ? slots.get(i0 + k * 1024, capacity) : capacity;
-    __syncthreads();
+        for (int k = 0; k < kSlotWide / 1024; ++k)
+            c[k] = i0 + k * 1024 < n ? slots.get(i0 + k * 1024, capacity) : capacity;
+        __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSlotWide / 1024; ++k)
-        if (c[k] < capacity) atomicMax(&last[c[k]], (int32_t)(i0 + k * 1024));
+        for (int k = 0; k < kSlotWide / 1024; ++k)
+            if (c[k] < capacity) atomicMax(&last[c[k]], (int32_t)(i0 + k * 1024));
+        if (n - base <= gridDim.x * kSlotWide) break;
+    }
     __syncthreads();
     for (uint32_t s = threadIdx.x; s < capacity; s += 1024)
         if (last[s] >= 0) atomicMax(&w.last[s], last[s]);
@@ -198,10 +205,12 @@ __global__ __launch_bounds__(1024) void slot_last_few_kernel(uint32_t n, RowIds<
 template <typename I>
 __global__ __launch_bounds__(256) void slot_last_each_kernel(uint32_t n, RowIds<I> slots, uint32_t capacity, SlotWork w) {
     if (slots_distinct(w)) return;
+    for (uint32_t t = blockIdx.x; t < w.tiles; t += gridDim.x) {
 #pragma unroll
-    for (int k = 0; k < kSlotTile / 256; ++k) {
-        const uint32_t i = blockIdx.x * kSlotTile + k * 256 + threadIdx.x, c = i < n ? slots.get(i, capacity) : capacity;
-        if (c < capacity) atomicMax(&w.last[c], (int32_t)i);
+        for (int k = 0; k < kSlotTile / 256; ++k) {
+            const uint32_t i = t * kSlotTile + k * 256 + threadIdx.x, c = i < n ? slots.get(i, capacity) : capacity;
+            if (c < capacity) atomicMax(&w.last[c], (int32_t)i);
+        }
     }
 }
 
@@ -410,11 +419,13 @@ static void launch(const CacheCall& c, hipStream_t s) {
         const SlotWork w = slot_work(c.ws, c.n);
         const uint32_t n = (uint32_t)c.n, cap = a.capacity;
         hipLaunchKernelGGL((slot_check_kernel<I>), dim3(w.tiles), dim3(256), 0, s, n, a.slots, cap, w);
+        const uint32_t wide = (n + kSlotWide - 1) / kSlotWide;
         if (cap <= kFewCapacity)
-            hipLaunchKernelGGL((slot_last_few_kernel<I>), dim3((n + kSlotWide - 1) / kSlotWide), dim3(1024), 0, s, n,
-                               a.slots, cap, w);
+            hipLaunchKernelGGL((slot_last_few_kernel<I>), dim3(wide < kSlotWideBlocks ? wide : kSlotWideBlocks), dim3(1024),
+                               0, s, n, a.slots, cap, w);
         else
-            hipLaunchKernelGGL((slot_last_each_kernel<I>), dim3(w.tiles), dim3(256), 0, s, n, a.slots, cap, w);
+            hipLaunchKernelGGL((slot_last_each_kernel<I>), dim3(w.tiles < kSlotBlocks ? w.tiles : kSlotBlocks), dim3(256), 0,
+                               s, n, a.slots, cap, w);
         a.last = w.last;
         a.distinct = w.distinct;
     }
