@@ -221,9 +221,10 @@ template <typename XT, typename I, int FMT, int VEC, bool FEW>
 __global__ __launch_bounds__(256) void rowcache_write_kernel(const CacheArgs<I> a) {
     __shared__ uint32_t key[FEW ? 2 * kFewSlots : 1];
     __shared__ int32_t last[FEW ? 2 * kFewSlots : 1];
-    // Narrow rows: an XCD's workgroups take consecutive ones, so that slots in order share its L2's lines
-    // (500k rows of 32 floats 24.5 us, 25.3 without).  Wide ones share none (16k of 2048: 41.8, 43.1 with).
-    const uint32_t c = (a.D < 128 ? xcd_remap(blockIdx.x, gridDim.x) : blockIdx.x) * 256 + threadIdx.x;
+    // An XCD's workgroups take consecutive rows, so that narrow rows' slots in order share its L2's lines
+    // (500k rows of 32 floats 24.5 us, 25.3 without); wide rows share none and take as long either way (16k of
+    // 2048 bf16 33.3 and 33.4 us, in order 27.6 and 28.1).
+    const uint32_t c = xcd_remap(blockIdx.x, gridDim.x) * 256 + threadIdx.x;
     const bool in = c < a.chunks;
     const uint32_t r = a.per_row.div(in ? c : 0);
     const int64_t row = a.row0 + r;
