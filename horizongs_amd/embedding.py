@@ -15,7 +15,6 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.graph import increment_version
 
 from . import _native as N
 from . import gradbuf
@@ -24,6 +23,9 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 _IDS = {torch.int32: 0, torch.int64: 1}
+
+# the calls behind torch.jit.is_tracing and torch.autograd.graph.increment_version (0.1 and 0.3 us less)
+_is_tracing, increment_version = torch._C._is_tracing, torch._C._increment_version
 
 
 def check_device(*ts):
@@ -80,7 +82,7 @@ def id_stride(flat):
 
 def refuse_trace():
     """torch.jit.trace would record the allocation of a result and not the call that fills it."""
-    if torch._C._get_tracing_state() is not None:
+    if _is_tracing():
         raise NotImplementedError("hgsr: calls on row tables cannot be traced")
 
 
@@ -90,19 +92,21 @@ def _recorded(t):
     return (t.requires_grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0
 
 
-def _lookup(weight, flat, shape, scale, dtype, index):
+def _lookup(weight, stride, flat, shape, scale, dtype, index):
     V, D = weight.shape
     out = weight.new_empty((*shape, D), dtype=dtype)
     n = flat.shape[0]
     if n and D:
         N.call_on(index, "hgsr_embed_fwd", V, n, D, weight.data_ptr(), _TYPES[weight.dtype],
-                  row_stride(weight, "weight"), flat.data_ptr(), _IDS[flat.dtype], id_stride(flat), scale,
+                  stride, flat.data_ptr(), _IDS[flat.dtype], id_stride(flat), scale,
                   out.data_ptr(), _TYPES[dtype])
     return out
 
 
-def _grad(grad, flat, out, scale, accumulate, index):
+def _grad(grad, flat, out, scale, index, added=None):
+    """The sums in out, which is contiguous, or added to out, whose rows lie `added` elements apart."""
     V, D = out.shape
+    accumulate = added is not None
     n = flat.shape[0]
     if V == 0 or D == 0 or (n == 0 and accumulate):
         return out
@@ -110,7 +114,7 @@ def _grad(grad, flat, out, scale, accumulate, index):
     ws = torch.empty(ws_b, dtype=torch.uint8, device=out.device) if ws_b else None
     N.call_on(index, "hgsr_embed_bwd", V, n, D, grad.data_ptr(), _TYPES[grad.dtype], row_stride(grad, "grad"),
               flat.data_ptr(), _IDS[flat.dtype], id_stride(flat), scale, out.data_ptr(), _TYPES[out.dtype],
-              row_stride(out, "out"), accumulate, ws.data_ptr() if ws_b else None, ws_b)
+              added if accumulate else D, accumulate, ws.data_ptr() if ws_b else None, ws_b)
     return out
 
 
@@ -119,7 +123,7 @@ class _Embedding(torch.autograd.Function):
     def forward(ctx, weight, flat, shape, scale, dtype, index):
         ctx.save_for_backward(flat)
         ctx.args = weight.shape, weight.dtype, (weight.data_ptr(), weight.numel()), scale, index
-        return _lookup(weight, flat, shape, scale, dtype, index)
+        return _lookup(weight, row_stride(weight, "weight"), flat, shape, scale, dtype, index)
 
     @staticmethod
     def backward(ctx, g):
@@ -131,7 +135,7 @@ class _Embedding(torch.autograd.Function):
         out = gradbuf.take(key, shape, dtype)  # in place in a DDP bucket when one is registered
         if out is None:
             out = g.new_empty(shape, dtype=dtype)
-        return _grad(rows_view(g, shape[1], "grad"), flat, out, scale, 0, index), None, None, None, None, None
+        return _grad(rows_view(g, shape[1], "grad"), flat, out, scale, index), None, None, None, None, None
 
 
 class _EmbeddingGrad(torch.autograd.Function):
@@ -139,7 +143,7 @@ class _EmbeddingGrad(torch.autograd.Function):
     def forward(ctx, g, flat, shape, dtype, scale, index):
         ctx.save_for_backward(flat)
         ctx.args = (g.shape, g.dtype, scale, index)
-        return _grad(rows_view(g, shape[1], "grad"), flat, g.new_empty(shape, dtype=dtype), scale, 0, index)
+        return _grad(rows_view(g, shape[1], "grad"), flat, g.new_empty(shape, dtype=dtype), scale, index)
 
     @staticmethod
     def backward(ctx, gg):
@@ -148,7 +152,7 @@ class _EmbeddingGrad(torch.autograd.Function):
         gg = rows_view(gg, gg.shape[1], "the gradient's gradient")
         if torch.is_grad_enabled() or _recorded(gg):
             return _Embedding.apply(gg, flat, shape[:-1], scale, dtype, index), None, None, None, None, None
-        return _lookup(gg, flat, shape[:-1], scale, dtype, index), None, None, None, None, None
+        return _lookup(gg, row_stride(gg, "weight"), flat, shape[:-1], scale, dtype, index), None, None, None, None, None
 
 
 def embedding(weight, ids, scale=1.0, dtype=None):
@@ -163,13 +167,13 @@ def embedding(weight, ids, scale=1.0, dtype=None):
         dtype = weight.dtype
     else:
         type_code(dtype)
-    row_stride(weight, "weight")
+    stride = row_stride(weight, "weight")
     check_ids(ids)
     index = check_device(weight, ids)
     flat = flat_ids(ids)
     if _recorded(weight):
         return _Embedding.apply(weight, flat, ids.shape, float(scale), dtype, index)
-    return _lookup(weight, flat, ids.shape, float(scale), dtype, index)
+    return _lookup(weight, stride, flat, ids.shape, float(scale), dtype, index)
 
 
 def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
@@ -194,22 +198,23 @@ def embedding_grad(grad, ids, num_rows, scale=1.0, dtype=None, out=None):
         index = check_device(grad, ids)
         if _recorded(grad):
             return _EmbeddingGrad.apply(grad, flat_ids(ids), (num_rows, D), dtype, float(scale), index)
-        out, accumulate = grad.new_empty((num_rows, D), dtype=dtype), 0
+        out, added = grad.new_empty((num_rows, D), dtype=dtype), None
     else:
         type_code(out.dtype)
         if tuple(out.shape) != (num_rows, D) or (dtype is not None and dtype != out.dtype):
             raise ValueError(f"hgsr: out is {tuple(out.shape)} of {out.dtype}, not {(num_rows, D)} of "
                              f"{dtype or 'its type'}")
-        if row_stride(out, "out") < D:
+        added = row_stride(out, "out")
+        if added < D:
             raise ValueError("hgsr: the rows of out overlap")
         if torch.is_grad_enabled() and (grad.requires_grad or out.requires_grad):
             raise NotImplementedError("hgsr: sums added to out are not differentiable (torch.no_grad())")
         if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (grad, out)):
             raise NotImplementedError("hgsr: sums added to out are not differentiable, in forward mode neither")
-        index, accumulate = check_device(grad, ids, out), 1
-    _grad(rows_view(grad, D, "grad"), flat_ids(ids), out, float(scale), accumulate, index)
-    if accumulate and grad.numel():
-        increment_version(out)  # a backward that saved out as it was must not go on with it
+        index = check_device(grad, ids, out)
+    _grad(rows_view(grad, D, "grad"), flat_ids(ids), out, float(scale), index, added)
+    if added is not None and grad.numel():
+        increment_version((out,))  # a backward that saved out as it was must not go on with it
     return out
 
 

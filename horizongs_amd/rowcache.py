@@ -19,10 +19,10 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.graph import increment_version
 
 from . import _native as N
-from .embedding import _TYPES, check_device, check_ids, id_stride, refuse_trace, row_stride, type_code
+from .embedding import (_TYPES, check_device, check_ids, id_stride, increment_version, refuse_trace, row_stride,
+                        type_code)
 
 _FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _NAMES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
@@ -55,13 +55,15 @@ def _cache(cache):
     if codes.dtype not in _FORMATS or codes.dim() != 2 or codes.shape[1] < 1:
         raise ValueError(f"hgsr row cache: codes {tuple(codes.shape)} of {codes.dtype}: [capacity, columns] of int8 or "
                          "float8_e4m3fn are needed")
-    if scales.dtype != torch.float32 or scales.shape != (codes.shape[0], -(-codes.shape[1] // group)):
+    capacity, dim = codes.shape
+    groups = -(-dim // group)
+    if scales.dtype != torch.float32 or scales.shape != (capacity, groups):
         raise ValueError(f"hgsr row cache: scales {tuple(scales.shape)} of {scales.dtype} do not fit codes "
                          f"{tuple(codes.shape)} in groups of {group}")
     cs, ss = row_stride(codes, "codes"), row_stride(scales, "scales")
-    if cs < codes.shape[1] or ss < scales.shape[1]:
+    if cs < dim or ss < groups:
         raise ValueError("hgsr row cache: its rows overlap")
-    return codes, scales, group, cs, ss
+    return codes, scales, group, capacity, dim, cs, ss
 
 
 def _slot_args(slots):
@@ -81,9 +83,8 @@ def rowcache_write(cache, rows, slots=None):
     int64 [n]; None: slots 0 .. n - 1).  A row whose slot lies outside the cache (-1 by custom) is left
     out; where a slot is named twice, the last of its rows stays.  Other slots keep what they hold.  A
     write is ordered on the current stream like any kernel; two streams must not write one slot at once."""
-    codes, scales, group, cs, ss = _cache(cache)
+    codes, scales, group, capacity, dim, cs, ss = _cache(cache)
     xt = type_code(rows.dtype)
-    capacity, dim = codes.shape
     if rows.dim() != 2 or rows.shape[1] != dim:
         raise ValueError(f"hgsr row cache: rows {tuple(rows.shape)}: [n, {dim}] are needed")
     n = rows.shape[0]
@@ -107,9 +108,8 @@ def rowcache_write(cache, rows, slots=None):
 def rowcache_read(cache, slots=None, dtype=torch.float32):
     """Rows [n, dim] of the named slots (int32 / int64 [n]; None: every slot) in `dtype`: code * scale in
     f32, rounded once.  A slot outside the cache reads zeros."""
-    codes, scales, group, cs, ss = _cache(cache)
+    codes, scales, group, capacity, dim, cs, ss = _cache(cache)
     ot = type_code(dtype)
-    capacity, dim = codes.shape
     if slots is None:
         n, index = capacity, check_device(codes, scales)
     else:
